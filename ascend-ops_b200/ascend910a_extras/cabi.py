@@ -9,13 +9,16 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_void_p
 
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG_DIR, "lib", "libb200ops.so")
 
 KV_LAYOUT_NZ = 0
 KV_LAYOUT_NHD = 1
+
+ROTARY_NONE, ROTARY_LINEAR, ROTARY_NTK, ROTARY_YARN, ROTARY_BANDS = range(5)
+TABLE_F16, TABLE_F32 = 0, 1
 
 OK = 0
 EINVAL = -1
@@ -64,6 +67,15 @@ SIGNATURES = {
     "b200ops_matmul": (c_int, [c_void_p] * 3 + [c_int64] * 3 + [c_void_p]),
     "b200ops_moe_dispatch": (c_int, [c_void_p] * 7 + [c_int64] * 2 + [c_void_p] * 6 + [c_int64] * 8 + [c_void_p]),
     "b200ops_moe_gather": (c_int, [c_void_p] * 8 + [c_int64] * 5 + [c_void_p]),
+    "b200ops_rotary_frequencies": (c_int, [c_int64, c_double, c_int, c_double, c_int64, c_double, c_double,
+                                           ctypes.POINTER(c_double), ctypes.POINTER(c_double)]),
+    "b200ops_rotary_tables": (c_int, [ctypes.POINTER(c_double), c_int64, c_double, c_int64, c_int64, c_void_p, c_void_p,
+                                      c_int, c_void_p]),
+    "b200ops_rotary": (c_int, [c_void_p] * 5 + [c_int] + [c_void_p] * 2 + [c_int64] * 8 + [c_int, c_void_p]),
+    "b200ops_copy_pages": (c_int, [ctypes.POINTER(c_void_p)] + [c_int64] * 3 + [c_void_p] * 2 + [c_int64, c_void_p]),
+    "b200ops_compact_pages_workspace_size": (c_size_t, [c_int64]),
+    "b200ops_compact_pages": (c_int, [ctypes.POINTER(c_void_p)] + [c_int64] * 3 + [c_void_p] * 2 + [c_int64] * 2 +
+                              [c_void_p] * 4 + [c_size_t, c_void_p]),
     "b200ops_moe_combine": (c_int, [c_void_p] * 7 + [c_int64] * 5 + [c_void_p]),
 }
 
@@ -189,6 +201,50 @@ def grouped_matmul_swiglu(x, w_storage, group_list, y, workspace=None, stream=No
 def matmul(x, w, y, stream=None):
     """y [m, n] = x [m, k] . w [n, k]^T (any m, n, k)."""
     check(load().b200ops_matmul(_ptr(x), _ptr(w), _ptr(y), x.shape[0], w.shape[0], x.shape[1], _stream(stream)))
+
+
+def rotary_frequencies(rotary_dim, base=10000.0, scaling=ROTARY_NONE, factor=1.0, original_positions=0, low=1.0,
+                       high=32.0):
+    """(list of rotary_dim/2 frequencies, amplitude); host arithmetic."""
+    f = (c_double * max(rotary_dim // 2, 1))()
+    a = c_double(0.0)
+    check(load().b200ops_rotary_frequencies(rotary_dim, base, scaling, factor, original_positions, low, high, f,
+                                            ctypes.byref(a)))
+    return list(f), a.value
+
+
+def rotary_tables(frequencies, amplitude, start, cos_table, sin_table, table_type, stream=None):
+    f = (c_double * len(frequencies))(*frequencies)
+    check(load().b200ops_rotary_tables(f, len(frequencies), amplitude, start, cos_table.shape[0], _ptr(cos_table),
+                                       _ptr(sin_table), table_type, _stream(stream)))
+
+
+def rotary(q, k, position_ids, cos_table, sin_table, table_type, out_q, out_k, interleaved, stream=None):
+    check(load().b200ops_rotary(_ptr(q), _ptr(k), _ptr(position_ids), _ptr(cos_table), _ptr(sin_table), table_type,
+                                _ptr(out_q), _ptr(out_k), q.shape[0], q.shape[1], k.shape[1], q.shape[2],
+                                2 * cos_table.shape[1], q.stride(0), k.stride(0), cos_table.shape[0],
+                                int(interleaved), _stream(stream)))
+
+
+def _pages(tensors):
+    table = (c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+    return table, len(tensors), tensors[0].shape[0], tensors[0][0].numel() * tensors[0].element_size()
+
+
+def copy_pages(tensors, src_pages, dst_pages, stream=None):
+    check(load().b200ops_copy_pages(*_pages(tensors), _ptr(src_pages), _ptr(dst_pages), src_pages.numel(),
+                                    _stream(stream)))
+
+
+def compact_pages_workspace_size(num_pages) -> int:
+    return load().b200ops_compact_pages_workspace_size(num_pages)
+
+
+def compact_pages(tensors, block_tables, page_counts, new_block_tables, page_map, num_live, workspace, stream=None):
+    ws_size = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    check(load().b200ops_compact_pages(*_pages(tensors), _ptr(block_tables), _ptr(page_counts), block_tables.shape[0],
+                                       block_tables.shape[1], _ptr(new_block_tables), _ptr(page_map), _ptr(num_live),
+                                       _ptr(workspace), ws_size, _stream(stream)))
 
 
 def reload_options() -> None:

@@ -77,3 +77,75 @@ def paged_attention(
 ) -> torch.Tensor:
     """Decode attention of q [B,Hq,D] over the paged KV cache; returns [B,Hq,D]."""
     return _C.ops.paged_attention(q, key_cache, value_cache, block_tables, context_lens)
+
+
+_ROTARY_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
+
+
+def rotary_frequencies(
+    rotary_dim: int,
+    base: float = 10000.0,
+    scaling: str = "none",
+    factor: float = 1.0,
+    original_positions: int = 0,
+    low: float | None = None,
+    high: float | None = None,
+) -> tuple[torch.Tensor, float]:
+    """Rotary frequencies, optionally scaled for longer contexts: (float64 CPU [rotary_dim/2],
+    amplitude), both for `rotary_tables`.  scaling: "none", "linear", "ntk", "yarn" (ramp between
+    `low`=1 and `high`=32 turns over `original_positions`) or "bands" (`low`=1, `high`=4)."""
+    if scaling not in _ROTARY_SCALINGS:
+        raise RuntimeError(f"rotary_frequencies: scaling must be one of {sorted(_ROTARY_SCALINGS)}, got {scaling!r}")
+    low = 1.0 if low is None else low
+    high = (4.0 if scaling == "bands" else 32.0) if high is None else high
+    return _C.ops.rotary_frequencies(
+        rotary_dim, base, _ROTARY_SCALINGS[scaling], factor, original_positions, low, high
+    )
+
+
+def rotary_tables(
+    frequencies: torch.Tensor,
+    num_positions: int,
+    amplitude: float = 1.0,
+    start: int = 0,
+    dtype: torch.dtype = torch.float16,
+    device: torch.device | str | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """(cos, sin) tables [num_positions, len(frequencies)] of positions start, start+1, ... on the
+    current CUDA device (or `device`), float16 (what `rope` takes) or float32."""
+    if device is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    else:
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+    return _C.ops.rotary_tables(frequencies, num_positions, amplitude, start, dtype, device)
+
+
+def rotary(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    position_ids: torch.Tensor,
+    cos_table: torch.Tensor,
+    sin_table: torch.Tensor,
+    interleaved: bool = False,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rotary embedding of q [T,Hq,D] and k [T,Hkv,D] with tables [max_pos, R/2], float16 or
+    float32: pairs (j, j+R/2), or (2j, 2j+1) if `interleaved`, of the first R channels; the
+    others are copied.  q and k may be views whose tokens are further apart than their heads."""
+    return _C.ops.rotary(q, k, position_ids, cos_table, sin_table, interleaved)
+
+
+def copy_pages(caches: list[torch.Tensor], src_pages: torch.Tensor, dst_pages: torch.Tensor) -> None:
+    """caches[i][dst_pages[j]] = caches[i][src_pages[j]] for j = 0, 1, ... in order, in place; pairs
+    that name no page are skipped.  `caches`: contiguous [pages, ...] tensors of any type."""
+    return _C.ops.copy_pages(list(caches), src_pages, dst_pages)
+
+
+def compact_pages(
+    caches: list[torch.Tensor], block_tables: torch.Tensor, page_counts: torch.Tensor
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Move the pages named by the first page_counts[b] entries of each row of block_tables to the
+    front of every cache, in place.  Returns (new block tables, page_map [pages]: the new number of
+    each live page, -1 for the others, num_live [1])."""
+    return _C.ops.compact_pages(list(caches), block_tables, page_counts)

@@ -685,6 +685,155 @@ at::Tensor moe_combine(at::Tensor returned, at::Tensor slot_to_row, at::Tensor e
   return y;
 }
 
+// ---- long contexts: rotary tables and embedding, cache pages (see include/b200ops.h) ----
+namespace {
+
+int table_type_of(at::ScalarType t, const char* op) {
+  TORCH_CHECK(t == at::kHalf || t == at::kFloat, op, ": tables must be float16 or float32, got ", t);
+  return t == at::kHalf ? B200OPS_TABLE_F16 : B200OPS_TABLE_F32;
+}
+
+// A [T, heads, D] tensor whose heads and channels are dense: the stride between tokens is free.
+void check_token_view(const at::Tensor& t, const char* op, const char* name) {
+  TORCH_CHECK((t.size(2) <= 1 || t.stride(2) == 1) && (t.size(1) <= 1 || t.stride(1) == t.size(2)) &&
+                  (t.size(0) <= 1 || t.stride(0) >= t.size(1) * t.size(2)),
+              op, ": the heads and channels of ", name, " must be contiguous within a token, got strides ", t.strides());
+}
+
+int64_t token_stride(const at::Tensor& t) {
+  return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2);
+}
+
+std::vector<void*> page_tensors(const std::vector<at::Tensor>& caches, const char* op, int64_t* num_pages,
+                                int64_t* page_bytes) {
+  TORCH_CHECK(!caches.empty(), op, ": at least one cache tensor is needed");
+  std::vector<void*> out;
+  out.reserve(caches.size());
+  for (const at::Tensor& t : caches) {
+    TORCH_CHECK(t.is_cuda(), op, ": caches must be CUDA tensors (there is no CPU path)");
+    TORCH_CHECK(t.dim() >= 2 && t.numel() > 0 && t.is_contiguous(), op,
+                ": caches must be contiguous tensors [pages, ...], got ", t.sizes());
+    TORCH_CHECK(t.device() == caches[0].device(), op, ": all tensors must be on the same device");
+    const int64_t bytes = t.numel() / t.size(0) * static_cast<int64_t>(t.element_size());
+    if (out.empty()) {
+      *num_pages = t.size(0);
+      *page_bytes = bytes;
+    }
+    TORCH_CHECK(t.size(0) == *num_pages && bytes == *page_bytes, op,
+                ": all caches must have the same number of pages and bytes per page");
+    out.push_back(t.data_ptr());
+  }
+  return out;
+}
+
+}  // namespace
+
+// Returns (frequencies float64 [rotary_dim/2] on the CPU, amplitude).
+std::tuple<at::Tensor, double> rotary_frequencies(int64_t rotary_dim, double base, int64_t scaling, double factor,
+                                                  int64_t original_positions, double low, double high) {
+  at::Tensor f = at::empty({std::max<int64_t>(rotary_dim, 0) / 2}, at::TensorOptions().dtype(at::kDouble));
+  double amplitude = 1.0;
+  check_status(b200ops_rotary_frequencies(rotary_dim, base, static_cast<int>(scaling), factor, original_positions, low,
+                                          high, f.data_ptr<double>(), &amplitude),
+               "rotary_frequencies");
+  return std::make_tuple(f, amplitude);
+}
+
+std::tuple<at::Tensor, at::Tensor> rotary_tables(at::Tensor frequencies, int64_t num_positions, double amplitude,
+                                                 int64_t start, at::ScalarType dtype, at::Device device) {
+  TORCH_CHECK(frequencies.device().is_cpu() && frequencies.scalar_type() == at::kDouble && frequencies.dim() == 1 &&
+                  frequencies.is_contiguous(),
+              "rotary_tables: frequencies must be a contiguous 1D float64 CPU tensor");
+  TORCH_CHECK(device.is_cuda(), "rotary_tables: device must be a CUDA device (there is no CPU path)");
+  TORCH_CHECK(num_positions >= 0, "rotary_tables: num_positions must not be negative, got ", num_positions);
+  const int type = table_type_of(dtype, "rotary_tables");
+  const c10::cuda::CUDAGuard guard(device);
+  const auto opt = at::TensorOptions().dtype(dtype).device(device);
+  at::Tensor c = at::empty({num_positions, frequencies.size(0)}, opt), s = at::empty_like(c);
+  check_status(b200ops_rotary_tables(frequencies.data_ptr<double>(), frequencies.size(0), amplitude, start,
+                                     num_positions, c.data_ptr(), s.data_ptr(), type, current_stream()),
+               "rotary_tables");
+  return std::make_tuple(c, s);
+}
+
+std::tuple<at::Tensor, at::Tensor> rotary(at::Tensor q, at::Tensor k, at::Tensor position_ids, at::Tensor cos_table,
+                                          at::Tensor sin_table, bool interleaved) {
+  TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && position_ids.dim() == 1 && cos_table.dim() == 2 && sin_table.dim() == 2,
+              "rotary: input tensors must be 3D, 3D, 1D, 2D, and 2D, got ", q.dim(), "D, ", k.dim(), "D, ",
+              position_ids.dim(), "D, ", cos_table.dim(), "D, ", sin_table.dim(), "D");
+  TORCH_CHECK(k.size(0) == q.size(0) && k.size(2) == q.size(2) && position_ids.size(0) == q.size(0),
+              "rotary: q, k and position_ids must agree in tokens and head_dim, got ", q.sizes(), ", ", k.sizes(),
+              " and ", position_ids.sizes());
+  check_f16_cuda(q, "rotary", "q");
+  check_f16_cuda(k, "rotary", "k");
+  check_i32_cuda(position_ids, "rotary", "position_ids");
+  check_token_view(q, "rotary", "q");
+  check_token_view(k, "rotary", "k");
+  TORCH_CHECK(cos_table.is_cuda() && sin_table.is_cuda() && cos_table.is_contiguous() && sin_table.is_contiguous() &&
+                  sin_table.scalar_type() == cos_table.scalar_type() && sin_table.sizes() == cos_table.sizes(),
+              "rotary: cos_table and sin_table must be contiguous CUDA tensors of one shape and type");
+  const int type = table_type_of(cos_table.scalar_type(), "rotary");
+  TORCH_CHECK(cos_table.size(1) >= 1 && 2 * cos_table.size(1) <= q.size(2),
+              "rotary: tables must be [max_pos, rotary_dim/2] with rotary_dim at most head_dim ", q.size(2), ", got ",
+              cos_table.sizes());
+  check_same_device(q, k, "rotary");
+  check_same_device(q, position_ids, "rotary");
+  check_same_device(q, cos_table, "rotary");
+  check_same_device(q, sin_table, "rotary");
+  const c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor out_q = at::empty(q.sizes(), q.options()), out_k = at::empty(k.sizes(), k.options());
+  check_status(b200ops_rotary(q.data_ptr(), k.data_ptr(), position_ids.data_ptr<int32_t>(), cos_table.data_ptr(),
+                              sin_table.data_ptr(), type, out_q.data_ptr(), out_k.data_ptr(), q.size(0), q.size(1),
+                              k.size(1), q.size(2), 2 * cos_table.size(1), token_stride(q), token_stride(k),
+                              cos_table.size(0), interleaved ? 1 : 0, current_stream()),
+               "rotary");
+  return std::make_tuple(out_q, out_k);
+}
+
+void copy_pages(std::vector<at::Tensor> caches, at::Tensor src_pages, at::Tensor dst_pages) {
+  int64_t num_pages = 0, page_bytes = 0;
+  std::vector<void*> tensors = page_tensors(caches, "copy_pages", &num_pages, &page_bytes);
+  check_i32_cuda(src_pages, "copy_pages", "src_pages");
+  check_i32_cuda(dst_pages, "copy_pages", "dst_pages");
+  TORCH_CHECK(src_pages.dim() == 1 && src_pages.sizes() == dst_pages.sizes(),
+              "copy_pages: src_pages and dst_pages must be 1D and of one length, got ", src_pages.sizes(), " and ",
+              dst_pages.sizes());
+  check_same_device(caches[0], src_pages, "copy_pages");
+  check_same_device(caches[0], dst_pages, "copy_pages");
+  const c10::cuda::CUDAGuard guard(caches[0].device());
+  check_status(b200ops_copy_pages(tensors.data(), static_cast<int64_t>(tensors.size()), num_pages, page_bytes,
+                                  src_pages.data_ptr<int32_t>(), dst_pages.data_ptr<int32_t>(), src_pages.numel(),
+                                  current_stream()),
+               "copy_pages");
+}
+
+// Returns (new block tables, page_map [pages], num_live [1]).
+std::tuple<at::Tensor, at::Tensor, at::Tensor> compact_pages(std::vector<at::Tensor> caches, at::Tensor block_tables,
+                                                             at::Tensor page_counts) {
+  int64_t num_pages = 0, page_bytes = 0;
+  std::vector<void*> tensors = page_tensors(caches, "compact_pages", &num_pages, &page_bytes);
+  check_i32_cuda(block_tables, "compact_pages", "block_tables");
+  check_i32_cuda(page_counts, "compact_pages", "page_counts");
+  TORCH_CHECK(block_tables.dim() == 2 && page_counts.dim() == 1 && page_counts.size(0) == block_tables.size(0),
+              "compact_pages: block_tables must be [sequences, pages] and page_counts [sequences], got ",
+              block_tables.sizes(), " and ", page_counts.sizes());
+  check_same_device(caches[0], block_tables, "compact_pages");
+  check_same_device(caches[0], page_counts, "compact_pages");
+  const c10::cuda::CUDAGuard guard(caches[0].device());
+  at::Tensor tables = at::empty(block_tables.sizes(), block_tables.options());
+  at::Tensor page_map = at::empty({num_pages}, block_tables.options());
+  at::Tensor num_live = at::empty({1}, block_tables.options());
+  const size_t ws = b200ops_compact_pages_workspace_size(num_pages);
+  at::Tensor workspace = at::empty({static_cast<int64_t>(ws)}, block_tables.options().dtype(at::kByte));
+  check_status(b200ops_compact_pages(tensors.data(), static_cast<int64_t>(tensors.size()), num_pages, page_bytes,
+                                     block_tables.data_ptr<int32_t>(), page_counts.data_ptr<int32_t>(),
+                                     block_tables.size(0), block_tables.size(1), tables.data_ptr<int32_t>(),
+                                     page_map.data_ptr<int32_t>(), num_live.data_ptr<int32_t>(), workspace.data_ptr(),
+                                     ws, current_stream()),
+               "compact_pages");
+  return std::make_tuple(tables, page_map, num_live);
+}
+
 void init_ffi_moe(py::module_&& m) {
   m.def("dispatch", &moe_dispatch, py::arg("x"), py::arg("router_weight"), py::arg("expert_ids"), py::arg("top_k"),
         py::arg("expert_slots"), py::arg("num_replicas"), py::arg("token_offset"), py::arg("peer_recv"),
@@ -720,6 +869,14 @@ void init_ffi_ops(py::module_&& m) {
   m.def("add_rms_norm", &add_rms_norm, "AddRMSNorm");
   m.def("reshape_and_cache", &reshape_and_cache, "ReshapeAndCache");
   m.def("paged_attention", &paged_attention, "PagedAttention");
+  m.def("rotary_frequencies", &rotary_frequencies, "Rotary frequencies (host)");
+  m.def("rotary_tables", [](at::Tensor f, int64_t n, double amplitude, int64_t start, py::object dtype, py::object device) {
+    return rotary_tables(f, n, amplitude, start, torch::python::detail::py_object_to_dtype(dtype),
+                         torch::python::detail::py_object_to_device(device));
+  }, "Rotary cos/sin tables");
+  m.def("rotary", &rotary, "Rotary embedding (half-split or interleaved, whole or part of the head)");
+  m.def("copy_pages", &copy_pages, "Copy cache pages");
+  m.def("compact_pages", &compact_pages, "Close the holes of a paged cache");
   m.def("matmul", &matmul, "MatMul (dense NT product of the reference's earlier interface)");
 }
 

@@ -396,6 +396,73 @@ int b200ops_moe_combine(const void* returned, const int32_t* slot_to_row, const 
                         int64_t row_elems, int64_t world, int64_t my_rank, void* stream);
 
 /*
+ * Rotary embeddings beyond b200ops_rope (no counterpart in the reference): interleaved pairs, a
+ * rotated part of each head, fp32 tables, and tables scaled for contexts longer than trained on.
+ *
+ * rotary_frequencies: host arithmetic in double, no CUDA call.  f_j = base^(-2j/rotary_dim) for
+ *   j < rotary_dim/2, scaled:
+ *     NONE    f_j
+ *     LINEAR  f_j / factor
+ *     NTK     base * factor^(rotary_dim/(rotary_dim-2)) in place of base
+ *     YARN    f_j / factor below index ceil(i(low)), f_j above floor(i(high)), linear in j between,
+ *             i(n) = the index that turns n times over original_positions; *amplitude = 0.1 ln(factor) + 1
+ *             (usual: low 1, high 32)
+ *     BANDS   share ((original_positions f_j / 2 pi) - low) / (high - low), clamped to [0, 1], of f_j,
+ *             the rest of f_j / factor (usual: low 1, high 4)
+ *   *amplitude is 1 except for YARN.  frequencies: double [rotary_dim/2], host memory; rotary_dim <= 512.
+ * rotary_tables: cos_table[p, j] = amplitude * cos((start + p) * frequencies[j]), sin_table likewise,
+ *   [num_positions, half] f16 or f32 (table_type).  `frequencies` is read on the host before the
+ *   call returns.  Angles are reduced in double: exact to the table's last bit at any position.
+ * rotary: q [num_tokens, num_heads, head_dim] and k [num_tokens, num_kv_heads, head_dim], f16, with
+ *   q_stride / k_stride elements from one token to the next (views of a packed projection);
+ *   out_q, out_k dense.  Tables [max_pos, rotary_dim/2] of table_type.  Pairs are (x[j], x[j + rotary_dim/2]),
+ *   or (x[2j], x[2j+1]) if `interleaved`; (a, b) -> (a cos - b sin, b cos + a sin); channels from
+ *   rotary_dim on are copied.  A position outside [0, max_pos) writes zeros, as in b200ops_rope.
+ *   The outputs may not overlap the inputs.
+ */
+#define B200OPS_ROTARY_NONE 0
+#define B200OPS_ROTARY_LINEAR 1
+#define B200OPS_ROTARY_NTK 2
+#define B200OPS_ROTARY_YARN 3
+#define B200OPS_ROTARY_BANDS 4
+#define B200OPS_TABLE_F16 0
+#define B200OPS_TABLE_F32 1
+int b200ops_rotary_frequencies(int64_t rotary_dim, double base, int scaling, double factor,
+                               int64_t original_positions, double low, double high, double* frequencies,
+                               double* amplitude);
+int b200ops_rotary_tables(const double* frequencies, int64_t half, double amplitude, int64_t start,
+                          int64_t num_positions, void* cos_table, void* sin_table, int table_type, void* stream);
+int b200ops_rotary(const void* q, const void* k, const int32_t* position_ids, const void* cos_table,
+                   const void* sin_table, int table_type, void* out_q, void* out_k, int64_t num_tokens,
+                   int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int64_t rotary_dim, int64_t q_stride,
+                   int64_t k_stride, int64_t max_pos, int interleaved, void* stream);
+
+/*
+ * Moving pages of the cache (no counterpart in the reference).  `tensors` is a HOST array of
+ * `num_tensors` (at most 1024) device pointers, each a tensor of num_pages pages of page_bytes
+ * contiguous bytes -- keys and values of any number of layers that share one page numbering, in
+ * either cache layout and any element type.  The tensors may not overlap.
+ *
+ * copy_pages: for i = 0, 1, ...: page dst_pages[i] = page src_pages[i], in every tensor; the result is
+ *   that of this loop, also where a page is named more than once.  Pairs that name no page (negative,
+ *   or >= num_pages) are skipped.  src_pages, dst_pages: device int32 [num_pairs].
+ * compact_pages: the live pages are those named by the first page_counts[b] entries of each row of
+ *   block_tables int32 [num_seqs, max_pages_per_seq] (entries that name no page are passed over; rows
+ *   may share pages).  With m of them, the live pages numbered >= m move, in ascending order, to the
+ *   numbers < m that are not live, in ascending order; no other page is written.  new_block_tables
+ *   (memory of its own) = the tables under the new numbers, entries not in use unchanged;
+ *   page_map int32 [num_pages] = new number of each live page, -1 for the others; num_live int32 [1] = m.
+ *   Everything is decided on the device.  num_pages <= 524288.  The workspace may hold anything.
+ */
+int b200ops_copy_pages(void* const* tensors, int64_t num_tensors, int64_t num_pages, int64_t page_bytes,
+                       const int32_t* src_pages, const int32_t* dst_pages, int64_t num_pairs, void* stream);
+size_t b200ops_compact_pages_workspace_size(int64_t num_pages);
+int b200ops_compact_pages(void* const* tensors, int64_t num_tensors, int64_t num_pages, int64_t page_bytes,
+                          const int32_t* block_tables, const int32_t* page_counts, int64_t num_seqs,
+                          int64_t max_pages_per_seq, int32_t* new_block_tables, int32_t* page_map,
+                          int32_t* num_live, void* workspace, size_t workspace_size, void* stream);
+
+/*
  * Health word of the pipelined kernels (grouped_matmul, paged_attention's TMA path).  Their
  * producer/consumer waits are bounded; a wait that runs out ends the kernel and leaves a
  * non-zero code here.  This call synchronises the device, returns the code in *status
