@@ -72,6 +72,8 @@ SIGNATURES = {
     "b200ops_rotary_tables": (c_int, [ctypes.POINTER(c_double), c_int64, c_double, c_int64, c_int64, c_void_p, c_void_p,
                                       c_int, c_void_p]),
     "b200ops_rotary": (c_int, [c_void_p] * 5 + [c_int] + [c_void_p] * 2 + [c_int64] * 8 + [c_int, c_void_p]),
+    "b200ops_chunked_paged_attention_workspace_size": (c_size_t, [c_int64] * 7),
+    "b200ops_chunked_paged_attention": (c_int, [c_void_p] * 7 + [c_int64] * 8 + [c_int, c_void_p, c_size_t, c_void_p]),
     "b200ops_copy_pages": (c_int, [ctypes.POINTER(c_void_p)] + [c_int64] * 3 + [c_void_p] * 2 + [c_int64, c_void_p]),
     "b200ops_compact_pages_workspace_size": (c_size_t, [c_int64]),
     "b200ops_compact_pages": (c_int, [ctypes.POINTER(c_void_p)] + [c_int64] * 3 + [c_void_p] * 2 + [c_int64] * 2 +
@@ -224,6 +226,22 @@ def rotary(q, k, position_ids, cos_table, sin_table, table_type, out_q, out_k, i
                                 _ptr(out_q), _ptr(out_k), q.shape[0], q.shape[1], k.shape[1], q.shape[2],
                                 2 * cos_table.shape[1], q.stride(0), k.stride(0), cos_table.shape[0],
                                 int(interleaved), _stream(stream)))
+
+
+def chunked_paged_attention_workspace_size(num_tokens, bs, num_heads, num_kv_heads, head_dim, page_size,
+                                           max_pages_per_seq) -> int:
+    return load().b200ops_chunked_paged_attention_workspace_size(num_tokens, bs, num_heads, num_kv_heads, head_dim,
+                                                                 page_size, max_pages_per_seq)
+
+
+def chunked_paged_attention(q, key_cache, value_cache, block_tables, context_lens, query_starts, out, num_kv_heads,
+                            page_size, layout, workspace, stream=None):
+    ws_size = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    check(load().b200ops_chunked_paged_attention(_ptr(q), _ptr(key_cache), _ptr(value_cache), _ptr(block_tables),
+                                                 _ptr(context_lens), _ptr(query_starts), _ptr(out), q.shape[0],
+                                                 context_lens.shape[0], q.shape[1], num_kv_heads, q.shape[2],
+                                                 key_cache.shape[0], page_size, block_tables.shape[1], layout,
+                                                 _ptr(workspace), ws_size, _stream(stream)))
 
 
 def _pages(tensors):

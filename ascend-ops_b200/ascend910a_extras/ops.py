@@ -136,6 +136,20 @@ def rotary(
     return _C.ops.rotary(q, k, position_ids, cos_table, sin_table, interleaved)
 
 
+def chunked_paged_attention(
+    q: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    query_starts: torch.Tensor,
+) -> torch.Tensor:
+    """Causal attention of the sequences' new tokens, q [T,Hq,D], over the paged KV cache that already
+    holds them.  Sequence b owns rows query_starts[b]..query_starts[b+1]-1 and has context_lens[b]
+    tokens in the cache, the new ones last.  Returns [T,Hq,D]; rows of no sequence are not written."""
+    return _C.ops.chunked_paged_attention(q, key_cache, value_cache, block_tables, context_lens, query_starts)
+
+
 def copy_pages(caches: list[torch.Tensor], src_pages: torch.Tensor, dst_pages: torch.Tensor) -> None:
     """caches[i][dst_pages[j]] = caches[i][src_pages[j]] for j = 0, 1, ... in order, in place; pairs
     that name no page are skipped.  `caches`: contiguous [pages, ...] tensors of any type."""

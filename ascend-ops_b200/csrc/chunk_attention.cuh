@@ -1,0 +1,137 @@
+// Shared definitions of the attention of chunks of new tokens over the paged KV cache: the work
+// list, the partial records of split contexts and their merge.
+//
+// Rows.  The query heads that share a kv head are folded into the rows of one matrix: row r of a
+// block is (token r / group, head r % group), so a key or value is read once for all of them and a
+// block of few tokens still fills the tensor core's rows.  Position of token i of a sequence with
+// n new tokens and L in its context: L - n + i; it sees the keys at positions 0 .. L - n + i.
+#pragma once
+
+#include "common.cuh"
+
+namespace b200ops {
+namespace ca {
+
+// One unit of work: `n_tok` tokens of one sequence, one tile of heads, a range of kv tiles.
+struct Item {
+  int q_tok;           // first token (row of q and out)
+  int n_tok;           // tokens of the block
+  int pos0;            // position of the first token in its sequence (negative: it sees nothing)
+  int seq;             // row of the block table
+  int head;            // kv head * head_tiles + tile of its query heads
+  int tile0, tile1;    // kv tiles; none if the block sees no key
+  int split, n_splits; // this range among those of the block (split >= n_splits: nothing to do)
+  int row0;            // partial rows of the block start here, those of split s at row0 + s * n_tok * group
+  int counter;         // index of the block's arrival counter (n_splits > 1)
+  int pad;
+};
+
+struct Header {
+  int n_items;
+  int ticket;  // next item to hand out
+};
+
+struct Args {
+  const __half* q;
+  const __half* k_cache;
+  const __half* v_cache;
+  const int32_t* block_tables;
+  const int32_t* context_lens;
+  const int32_t* query_starts;
+  __half* out;
+  // workspace
+  Header* header;
+  Item* items;
+  int* counters;
+  int* prefix;       // [bs + 1] items before each sequence, then the per-sequence plan
+  float* part_o;     // [rows, head_dim] un-normalised sums of a split
+  float2* part_ml;   // [rows] maximum (in base-2 units) and sum
+  int num_tokens, bs, num_heads, num_kv_heads, head_dim;
+  int num_pages, page_size, max_pages_per_seq, layout;
+  float scale_log2;  // 1/sqrt(head_dim) * log2(e)
+  // plan
+  int block_tokens;  // tokens per block
+  int kv_tile;       // tokens per kv tile
+  int group;         // query heads per tile of heads (rows per token)
+  int head_tiles;    // tiles of heads per kv head
+  int min_tiles;     // a split is at least this many kv tiles
+  int target;        // items wanted at least
+  int max_items, max_split_items, max_rows;
+};
+
+#ifdef __CUDACC__
+// Non-finite values among hidden keys.  A hidden key's probability is exactly 0, but the matrix
+// product still forms 0 * v, which is NaN if v is infinite or NaN.  So in kv tiles that some row of
+// the block does not see whole, such values are taken out of the V tile and remembered here --
+// per channel the first position that holds +inf, -inf and NaN -- and added to the sums of the
+// rows that do see them.
+constexpr int kNever = 0x7fffffff;
+
+__device__ __forceinline__ bool any_nonfinite(const uint4& v) {
+  auto hit = [&](uint32_t w) { return ((w & 0x7c00u) == 0x7c00u) || ((w & 0x7c000000u) == 0x7c000000u); };
+  return hit(v.x) || hit(v.y) || hit(v.z) || hit(v.w);
+}
+
+// Takes the non-finite halfs out of `v` (channels d .. d+7 of position t); `special` [3][head_dim].
+__device__ __noinline__ void take_nonfinite(uint4& v, int t, int d, int head_dim, int* special, int* flag) {
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t h = (w[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+    if ((h & 0x7c00u) != 0x7c00u) continue;
+    const int kind = (h & 0x3ffu) ? 2 : ((h & 0x8000u) ? 1 : 0);
+    atomicMin(&special[kind * head_dim + d + i], t);
+    w[i >> 1] &= ~(0xffffu << (16 * (i & 1)));
+    *flag = 1;
+  }
+  v = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// What a row at position `pos` adds to channel d for the values taken out.
+__device__ __forceinline__ float special_term(const int* special, int head_dim, int d, int pos) {
+  float s = 0.f;
+  if (special[d] <= pos) s += INFINITY;
+  if (special[head_dim + d] <= pos) s -= INFINITY;
+  if (special[2 * head_dim + d] <= pos) s = NAN;
+  return s;
+}
+
+// Merges the splits of one row (one warp) and stores the fp16 row.  The records were written by
+// other SMs of the same launch: ld.global.cg.
+__device__ __forceinline__ void merge_row(const Args& a, int row0, int rows, int r, int n_splits, __half* out, int lane) {
+  const float2* ml = a.part_ml + row0 + r;
+  float m = -INFINITY;
+  for (int s = lane; s < n_splits; s += 32) m = fmaxf(m, __ldcg(&ml[static_cast<size_t>(s) * rows].x));
+  m = warp_max(m);
+  const float m_use = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  for (int s = lane; s < n_splits; s += 32) {
+    const float2 v = __ldcg(&ml[static_cast<size_t>(s) * rows]);
+    l += v.y * exp2f(v.x - m_use);
+  }
+  l = warp_sum(l);
+  const float inv = l == 0.f ? 0.f : 1.0f / l;  // nothing visible: zeros; a NaN sum stays NaN
+  const int per = a.head_dim >> 5;  // channels lane, lane + 32, ...
+  float acc[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+  for (int s = 0; s < n_splits; ++s) {
+    const float w = exp2f(__ldcg(&ml[static_cast<size_t>(s) * rows].x) - m_use);
+    const float* o = a.part_o + (static_cast<size_t>(row0) + static_cast<size_t>(s) * rows + r) * a.head_dim;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < per) {
+        const float v = __ldcg(o + lane + 32 * i);
+        if (w != 0.f) acc[i] = fmaf(w, v, acc[i]);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < per) out[lane + 32 * i] = __float2half_rn(acc[i] * inv);
+}
+#endif
+
+int launch_plan(const Args& a, cudaStream_t st);
+int launch_general(const Args& a, cudaStream_t st);
+
+}  // namespace ca
+}  // namespace b200ops

@@ -790,6 +790,62 @@ std::tuple<at::Tensor, at::Tensor> rotary(at::Tensor q, at::Tensor k, at::Tensor
   return std::make_tuple(out_q, out_k);
 }
 
+at::Tensor chunked_paged_attention(at::Tensor q, at::Tensor key_cache, at::Tensor value_cache, at::Tensor block_tables,
+                                   at::Tensor context_lens, at::Tensor query_starts) {
+  const char* op = "chunked_paged_attention";
+  TORCH_CHECK(q.dim() == 3 && key_cache.dim() == 4 && value_cache.dim() == 4 && block_tables.dim() == 2 &&
+                  context_lens.dim() == 1 && query_starts.dim() == 1,
+              "chunked_paged_attention: q must be 3D, caches 4D, block_tables 2D, context_lens and query_starts 1D");
+  TORCH_CHECK(q.is_contiguous() && key_cache.is_contiguous() && value_cache.is_contiguous(),
+              "chunked_paged_attention: all input tensors must be contiguous");
+  check_f16_cuda(q, op, "q");
+  check_f16_cuda(key_cache, op, "key_cache");
+  check_f16_cuda(value_cache, op, "value_cache");
+  check_i32_cuda(block_tables, op, "block_tables");
+  check_i32_cuda(context_lens, op, "context_lens");
+  check_i32_cuda(query_starts, op, "query_starts");
+  TORCH_CHECK(value_cache.sizes() == key_cache.sizes(),
+              "chunked_paged_attention: key_cache and value_cache must have the same shape, got ", key_cache.sizes(),
+              " and ", value_cache.sizes());
+  TORCH_CHECK(block_tables.size(0) == context_lens.size(0) && query_starts.size(0) == context_lens.size(0) + 1,
+              "chunked_paged_attention: block_tables and context_lens must have one row per sequence, query_starts "
+              "one more, got ", block_tables.sizes(), ", ", context_lens.sizes(), " and ", query_starts.sizes());
+  check_same_device(q, key_cache, op);
+  check_same_device(q, value_cache, op);
+  check_same_device(q, block_tables, op);
+  check_same_device(q, context_lens, op);
+  check_same_device(q, query_starts, op);
+  const int64_t head_dim = q.size(2);
+  int layout;
+  int64_t num_kv_heads, page_size;
+  if (key_cache.size(3) == head_dim) {
+    layout = B200OPS_KV_LAYOUT_NHD;
+    page_size = key_cache.size(1);
+    num_kv_heads = key_cache.size(2);
+  } else {
+    TORCH_CHECK(head_dim > 0 && key_cache.size(3) == 16 && (key_cache.size(1) * 16) % head_dim == 0,
+                "chunked_paged_attention: cache must be [pages, Hkv*D/16, page_size, 16] or "
+                "[pages, page_size, Hkv, D], got ", key_cache.sizes());
+    layout = B200OPS_KV_LAYOUT_NZ;
+    num_kv_heads = key_cache.size(1) * 16 / head_dim;
+    page_size = key_cache.size(2);
+  }
+  const int64_t tokens = q.size(0), bs = context_lens.size(0);
+  const c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor y = at::empty_like(q);
+  const size_t ws = b200ops_chunked_paged_attention_workspace_size(tokens, bs, q.size(1), num_kv_heads, head_dim,
+                                                                   page_size, block_tables.size(1));
+  at::Tensor workspace = at::empty({static_cast<int64_t>(ws)}, q.options().dtype(at::kByte));
+  check_status(b200ops_chunked_paged_attention(q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+                                               block_tables.data_ptr<int32_t>(), context_lens.data_ptr<int32_t>(),
+                                               query_starts.data_ptr<int32_t>(), y.data_ptr(), tokens, bs, q.size(1),
+                                               num_kv_heads, head_dim, key_cache.size(0), page_size,
+                                               block_tables.size(1), layout, ws ? workspace.data_ptr() : nullptr, ws,
+                                               current_stream()),
+               op);
+  return y;
+}
+
 void copy_pages(std::vector<at::Tensor> caches, at::Tensor src_pages, at::Tensor dst_pages) {
   int64_t num_pages = 0, page_bytes = 0;
   std::vector<void*> tensors = page_tensors(caches, "copy_pages", &num_pages, &page_bytes);
@@ -875,6 +931,7 @@ void init_ffi_ops(py::module_&& m) {
                          torch::python::detail::py_object_to_device(device));
   }, "Rotary cos/sin tables");
   m.def("rotary", &rotary, "Rotary embedding (half-split or interleaved, whole or part of the head)");
+  m.def("chunked_paged_attention", &chunked_paged_attention, "Attention of new tokens over the paged cache");
   m.def("copy_pages", &copy_pages, "Copy cache pages");
   m.def("compact_pages", &compact_pages, "Close the holes of a paged cache");
   m.def("matmul", &matmul, "MatMul (dense NT product of the reference's earlier interface)");

@@ -438,6 +438,34 @@ int b200ops_rotary(const void* q, const void* k, const int32_t* position_ids, co
                    int64_t k_stride, int64_t max_pos, int interleaved, void* stream);
 
 /*
+ * Attention of chunks of new tokens over the paged KV cache: prompts read in one or several
+ * chunks, several tokens per sequence at once, or single tokens, mixed in one call (no counterpart
+ * in the reference; b200ops_paged_attention takes one token per sequence).
+ *   q, out : f16 [num_tokens, num_heads, head_dim], the sequences' new tokens one after the other;
+ *   query_starts : int32 [bs + 1], sequence b owns rows query_starts[b] .. query_starts[b+1] - 1;
+ *   context_lens : int32 [bs], tokens of the sequence in the cache, its new ones (already stored) included;
+ *   block_tables : int32 [bs, max_pages_per_seq]; caches in `layout`, num_pages pages of page_size tokens.
+ * Token i of a sequence with n new tokens and L in context stands at position p = L - n + i and
+ *   out = softmax(q . K[0..p]^T / sqrt(head_dim)) . V[0..p]   (query heads share kv heads as in paged_attention)
+ * A token with p < 0 gets zeros.  A block-table entry outside [0, num_pages) leaves its page's tokens out.
+ * A context above max_pages_per_seq * page_size is taken as that.  Rows that belong to no sequence are
+ * not written.  query_starts must not decrease (rows outside [0, num_tokens) are left out).
+ * What lies in the cache behind a token's position -- unused slots, other tokens of the chunk -- has no
+ * influence on its row, also if it is infinite or NaN.
+ * head_dim in {32, 64, 128, 256}; num_tokens <= 2^24.  Lengths are read on the device only, so a captured
+ * graph serves any lengths of its shape.  Results do not depend on scheduling (bitwise repeatable).
+ */
+size_t b200ops_chunked_paged_attention_workspace_size(int64_t num_tokens, int64_t bs, int64_t num_heads,
+                                                      int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
+                                                      int64_t max_pages_per_seq);
+int b200ops_chunked_paged_attention(const void* q, const void* key_cache, const void* value_cache,
+                                    const int32_t* block_tables, const int32_t* context_lens,
+                                    const int32_t* query_starts, void* out, int64_t num_tokens, int64_t bs,
+                                    int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int64_t num_pages,
+                                    int64_t page_size, int64_t max_pages_per_seq, int layout, void* workspace,
+                                    size_t workspace_size, void* stream);
+
+/*
  * Moving pages of the cache (no counterpart in the reference).  `tensors` is a HOST array of
  * `num_tensors` (at most 1024) device pointers, each a tensor of num_pages pages of page_bytes
  * contiguous bytes -- keys and values of any number of layers that share one page numbering, in

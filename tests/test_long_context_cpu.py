@@ -92,6 +92,23 @@ def test_page_refusals(cabi):
     assert compact(pages=524289) == cabi.EUNSUPPORTED
 
 
+def test_chunked_attention_refusals(cabi):
+    lib = cabi.load()
+    size = lib.b200ops_chunked_paged_attention_workspace_size
+    need = size(64, 2, 8, 2, 128, 16, 64)
+    assert need > 0 and size(0, 2, 8, 2, 128, 16, 64) == 0 and size(64, 2, 8, 3, 128, 16, 64) == 0
+    def att(tokens=64, bs=2, hq=8, hkv=2, d=128, pages=100, page=16, width=64, layout=1, ws=ONE, n=need, q=ONE):
+        return lib.b200ops_chunked_paged_attention(q, ONE, ONE, ONE, ONE, ONE, ONE, tokens, bs, hq, hkv, d, pages, page,
+                                                   width, layout, ws, n, NULL)
+    assert att(hkv=3) == cabi.EINVAL and "multiple of num_kv_heads" in cabi.last_error()
+    assert att(d=96) == cabi.EINVAL and "head_dim" in cabi.last_error()
+    assert att(layout=2) == cabi.EINVAL and att(pages=0) == cabi.EINVAL and att(page=0) == cabi.EINVAL
+    assert att(tokens=-1) == cabi.EINVAL and att(bs=70000) == cabi.EINVAL and att(tokens=1 << 25) == cabi.EINVAL
+    assert att(q=NULL) == cabi.EINVAL and att(q=ctypes.c_void_p(264)) == cabi.EINVAL
+    assert att(ws=NULL) == cabi.EWORKSPACE and att(n=need - 1) == cabi.EWORKSPACE
+    assert att(tokens=0) == cabi.OK and att(bs=0) == cabi.OK
+
+
 def test_python_layer_refusals(ops):
     q, pos = torch.zeros(2, 4, 64).half(), torch.zeros(2, dtype=torch.int32)
     tab = torch.zeros(8, 32).half()
@@ -111,6 +128,11 @@ def test_python_layer_refusals(ops):
         ops.rotary_frequencies(64, scaling="other")
     with pytest.raises(RuntimeError, match="factor"):
         ops.rotary_frequencies(64, scaling="linear", factor=0.0)
+    c = torch.zeros(4, 16, 2, 64).half()
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.chunked_paged_attention(q, c, c, pos[None], pos[:1], pos)
+    with pytest.raises(RuntimeError, match="4D"):
+        ops.chunked_paged_attention(q, c[0], c, pos[None], pos[:1], pos)
     f, a = ops.rotary_frequencies(64)
     assert f.dtype == torch.float64 and f.shape == (32,) and a == 1.0
     with pytest.raises(RuntimeError, match="CUDA device"):
