@@ -168,8 +168,9 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_attention_plan_kernel(Args
     it.seq = lo;
     it.head = head;
     const int tiles = (max(min(it.pos0 + it.n_tok, s.len), 0) + a.kv_tile - 1) / a.kv_tile;
-    it.n_splits = p.splits > 1 ? max(1, min(p.splits, (tiles + range - 1) / range)) : 1;
-    const int per = (tiles + it.n_splits - 1) / it.n_splits;
+    const int cut = p.splits > 1 ? max(1, min(p.splits, (tiles + range - 1) / range)) : 1;
+    const int per = max((tiles + cut - 1) / cut, 1);
+    it.n_splits = max((tiles + per - 1) / per, 1);  // no split is empty
     it.split = split;
     it.tile0 = min(split * per, tiles);
     it.tile1 = min(it.tile0 + per, tiles);
@@ -199,6 +200,31 @@ __device__ __forceinline__ size_t kv_offset(const Args& a, int page, int off, in
   const int e = head * a.head_dim + d;
   const size_t chunks = static_cast<size_t>(a.num_kv_heads) * a.head_dim / 16;
   return ((static_cast<size_t>(page) * chunks + (e >> 4)) * a.page_size + off) * 16 + (e & 15);
+}
+
+// Takes the non-finite halfs out of `v` (channels d .. d+7 of position t); `special` [3][head_dim].
+constexpr int kNever = 0x7fffffff;
+
+__device__ __noinline__ void take_nonfinite(uint4& v, int t, int d, int head_dim, int* special, int* flag) {
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t h = (w[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+    if ((h & 0x7c00u) != 0x7c00u) continue;
+    const int kind = (h & 0x3ffu) ? 2 : ((h & 0x8000u) ? 1 : 0);
+    atomicMin(&special[kind * head_dim + d + i], t);
+    w[i >> 1] &= ~(0xffffu << (16 * (i & 1)));
+    *flag = 1;
+  }
+  v = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// What a row at position `pos` adds to channel d for the values taken out.
+__device__ __forceinline__ float special_term(const int* special, int head_dim, int d, int pos) {
+  float s = 0.f;
+  if (special[d] <= pos) s += INFINITY;
+  if (special[head_dim + d] <= pos) s -= INFINITY;
+  if (special[2 * head_dim + d] <= pos) s = NAN;
+  return s;
 }
 
 // Four warps, each 16 of the block's 64 rows; K and V tiles go through shared memory, the products
@@ -266,7 +292,6 @@ __global__ void __launch_bounds__(kThreads) chunk_attention_general_kernel(Args 
 
     for (int tile = it.tile0; tile < it.tile1; ++tile) {
       const int t0 = tile * kTile;
-      const bool hidden = t0 + kTile - 1 > it.pos0;  // some row does not see the whole tile
       __syncthreads();
       if (tid < 64) {
         bool ok = false;
@@ -286,7 +311,7 @@ __global__ void __launch_bounds__(kThreads) chunk_attention_general_kernel(Args 
             const size_t off = kv_offset(a, page, (t0 + r) % a.page_size, kvh, c * 8);
             kv = *reinterpret_cast<const uint4*>(a.k_cache + off);
             vv = *reinterpret_cast<const uint4*>(a.v_cache + off);
-            if (hidden && any_nonfinite(vv)) take_nonfinite(vv, t0 + r, c * 8, D, special, &s_special);
+            if (t0 + r > it.pos0 && any_nonfinite(vv)) take_nonfinite(vv, t0 + r, c * 8, D, special, &s_special);
           }
         }
         *reinterpret_cast<uint4*>(sk + r * kLd + c * 8) = kv;
@@ -425,14 +450,23 @@ int launch_general_d(const Args& a, cudaStream_t st) {
 size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 // Everything of the plan that follows from the shape.
-void plan_shape(Args* a) {
+void plan_shape(Args* a, bool tc) {
   const int group = a->num_heads / a->num_kv_heads;
-  a->group = group < kRows ? group : kRows;
-  a->head_tiles = (group + a->group - 1) / a->group;
-  a->block_tokens = kRows / a->group;
-  a->kv_tile = a->head_dim == 256 ? 32 : 64;
-  a->min_tiles = 8;
-  a->target = 3 * sm_count();
+  if (tc) {  // two score tiles of 128 rows per block
+    a->group = group;
+    a->head_tiles = 1;
+    a->block_tokens = 2 * (128 / group);
+    a->kv_tile = 128;
+    a->min_tiles = 4;
+    a->target = 2 * sm_count();
+  } else {
+    a->group = group < kRows ? group : kRows;
+    a->head_tiles = (group + a->group - 1) / a->group;
+    a->block_tokens = kRows / a->group;
+    a->kv_tile = a->head_dim == 256 ? 32 : 64;
+    a->min_tiles = 8;
+    a->target = 3 * sm_count();
+  }
   const int64_t heads = static_cast<int64_t>(a->num_kv_heads) * a->head_tiles;
   const int64_t blocks = (a->num_tokens / a->block_tokens + static_cast<int64_t>(a->bs < a->num_tokens ? a->bs : a->num_tokens)) * heads;
   const int64_t cap_tiles = (static_cast<int64_t>(a->max_pages_per_seq) * a->page_size + a->kv_tile - 1) / a->kv_tile;
@@ -505,7 +539,7 @@ int check_shape(int64_t num_tokens, int64_t bs, int64_t num_heads, int64_t num_k
 }
 
 Args shape_args(int64_t num_tokens, int64_t bs, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
-                int64_t page_size, int64_t max_pages_per_seq) {
+                int64_t page_size, int64_t max_pages_per_seq, bool tc) {
   Args a = {};
   a.num_tokens = (int)num_tokens;
   a.bs = (int)bs;
@@ -514,7 +548,7 @@ Args shape_args(int64_t num_tokens, int64_t bs, int64_t num_heads, int64_t num_k
   a.head_dim = (int)head_dim;
   a.page_size = (int)page_size;
   a.max_pages_per_seq = (int)max_pages_per_seq;
-  plan_shape(&a);
+  plan_shape(&a, tc);
   return a;
 }
 
@@ -529,8 +563,14 @@ extern "C" size_t b200ops_chunked_paged_attention_workspace_size(int64_t num_tok
   if (ca::check_shape(num_tokens, bs, num_heads, num_kv_heads, head_dim, page_size, max_pages_per_seq) != B200OPS_OK ||
       num_tokens == 0 || bs == 0)
     return 0;
-  ca::Args a = ca::shape_args(num_tokens, bs, num_heads, num_kv_heads, head_dim, page_size, max_pages_per_seq);
-  return ca::lay_out(&a, nullptr);
+  ca::Args a = ca::shape_args(num_tokens, bs, num_heads, num_kv_heads, head_dim, page_size, max_pages_per_seq, false);
+  size_t need = ca::lay_out(&a, nullptr);
+  if (ca::tc_supported(head_dim, num_heads / num_kv_heads, page_size, B200OPS_KV_LAYOUT_NHD)) {
+    a = ca::shape_args(num_tokens, bs, num_heads, num_kv_heads, head_dim, page_size, max_pages_per_seq, true);
+    const size_t tc = ca::lay_out(&a, nullptr);
+    if (tc > need) need = tc;  // enough for either kernel: the layout and the option are not known here
+  }
+  return need;
 }
 
 extern "C" int b200ops_chunked_paged_attention(const void* q, const void* key_cache, const void* value_cache,
@@ -551,7 +591,8 @@ extern "C" int b200ops_chunked_paged_attention(const void* q, const void* key_ca
                   "chunked_paged_attention: null pointer");
   B200OPS_REQUIRE(aligned16(q) && aligned16(key_cache) && aligned16(value_cache) && aligned16(out),
                   "chunked_paged_attention: pointers must be 16-byte aligned");
-  ca::Args a = ca::shape_args(num_tokens, bs, num_heads, num_kv_heads, head_dim, page_size, max_pages_per_seq);
+  const bool tc = knob(kKnobPaMode, 0) != 2 && ca::tc_supported(head_dim, num_heads / num_kv_heads, page_size, layout);
+  ca::Args a = ca::shape_args(num_tokens, bs, num_heads, num_kv_heads, head_dim, page_size, max_pages_per_seq, tc);
   const size_t need = ca::lay_out(&a, static_cast<char*>(workspace));
   if (workspace == nullptr || workspace_size < need)
     return fail(B200OPS_EWORKSPACE, "chunked_paged_attention: workspace of %zu bytes needed, got %zu", need,
@@ -569,5 +610,6 @@ extern "C" int b200ops_chunked_paged_attention(const void* q, const void* key_ca
   a.scale_log2 = (1.0f / std::sqrt(static_cast<float>(head_dim))) * 1.44269504088896340736f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int pr = ca::launch_plan(a, st);
-  return pr != B200OPS_OK ? pr : ca::launch_general(a, st);
+  if (pr != B200OPS_OK) return pr;
+  return tc ? ca::launch_tc(a, st) : ca::launch_general(a, st);
 }

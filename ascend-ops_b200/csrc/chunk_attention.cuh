@@ -61,38 +61,12 @@ struct Args {
 
 #ifdef __CUDACC__
 // Non-finite values among hidden keys.  A hidden key's probability is exactly 0, but the matrix
-// product still forms 0 * v, which is NaN if v is infinite or NaN.  So in kv tiles that some row of
-// the block does not see whole, such values are taken out of the V tile and remembered here --
-// per channel the first position that holds +inf, -inf and NaN -- and added to the sums of the
-// rows that do see them.
-constexpr int kNever = 0x7fffffff;
-
+// product still forms 0 * v, which is NaN if v is infinite or NaN.  So the kernels take such values
+// out of the V tiles at positions that some row of the block does not see, remember per channel the
+// first position that holds +inf, -inf and NaN, and add them to the sums of the rows that do see them.
 __device__ __forceinline__ bool any_nonfinite(const uint4& v) {
   auto hit = [&](uint32_t w) { return ((w & 0x7c00u) == 0x7c00u) || ((w & 0x7c000000u) == 0x7c000000u); };
   return hit(v.x) || hit(v.y) || hit(v.z) || hit(v.w);
-}
-
-// Takes the non-finite halfs out of `v` (channels d .. d+7 of position t); `special` [3][head_dim].
-__device__ __noinline__ void take_nonfinite(uint4& v, int t, int d, int head_dim, int* special, int* flag) {
-  uint32_t w[4] = {v.x, v.y, v.z, v.w};
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t h = (w[i >> 1] >> (16 * (i & 1))) & 0xffffu;
-    if ((h & 0x7c00u) != 0x7c00u) continue;
-    const int kind = (h & 0x3ffu) ? 2 : ((h & 0x8000u) ? 1 : 0);
-    atomicMin(&special[kind * head_dim + d + i], t);
-    w[i >> 1] &= ~(0xffffu << (16 * (i & 1)));
-    *flag = 1;
-  }
-  v = make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-// What a row at position `pos` adds to channel d for the values taken out.
-__device__ __forceinline__ float special_term(const int* special, int head_dim, int d, int pos) {
-  float s = 0.f;
-  if (special[d] <= pos) s += INFINITY;
-  if (special[head_dim + d] <= pos) s -= INFINITY;
-  if (special[2 * head_dim + d] <= pos) s = NAN;
-  return s;
 }
 
 // Merges the splits of one row (one warp) and stores the fp16 row.  The records were written by
@@ -132,6 +106,8 @@ __device__ __forceinline__ void merge_row(const Args& a, int row0, int rows, int
 
 int launch_plan(const Args& a, cudaStream_t st);
 int launch_general(const Args& a, cudaStream_t st);
+bool tc_supported(int64_t head_dim, int64_t group, int64_t page_size, int layout);
+int launch_tc(const Args& a, cudaStream_t st);
 
 }  // namespace ca
 }  // namespace b200ops

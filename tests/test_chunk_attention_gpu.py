@@ -112,6 +112,12 @@ def call(ops, s):
     return ops.chunked_paged_attention(s["q"], s["kc"], s["vc"], s["table"], s["ctx"], s["starts"])
 
 
+@pytest.fixture(autouse=True)
+def _no_wait_ran_out(cabi):
+    yield
+    assert cabi.pipeline_status() == 0
+
+
 def check(got, s):
     want, tol = reference(s)
     owned = ~want.isnan()
@@ -282,6 +288,16 @@ def test_guards_around_output_and_workspace(cabi):
     assert bool((raw[:4096] == 0x7B3C).all()) and bool((raw[4096 + n:] == 0x7B3C).all())
     assert bool((ws[:4096] == 0x5C).all()) and bool((ws[4096 + need:] == 0x5C).all())
     check(out, s)
+
+
+@pytest.mark.parametrize("hq,hkv,d,page", [(28, 4, 128, 128), (8, 2, 64, 8), (128, 1, 128, 32)])
+def test_general_kernel_on_the_same_shapes(ops, monkeypatch, hq, hkv, d, page):
+    s = make([(33, 290), (1, 2000), (70, 70), (2, 1)], hq, hkv, d, page, seed=21)
+    fast = call(ops, s)
+    knob(monkeypatch, "B200OPS_PA_MODE", 2)
+    general = call(ops, s)
+    check(fast, s)
+    check(general, s)
 
 
 def test_many_sequences(ops):
