@@ -54,7 +54,10 @@ struct Shape {
 struct Meta {
   uint64_t item_full[2], item_empty[2];
   uint64_t q_full, q_empty;
-  uint64_t kv_full[10], kv_empty[10], v_ok[10];
+  // A stage holds a K or a V tile in turn.  Each kind has arrival barriers of its own, because the guard
+  // warps follow the V tiles alone and a copy may land long after ones issued behind it: with one
+  // barrier per stage they could take the tile before theirs for theirs.
+  uint64_t k_full[10], v_full[10], kv_empty[10], v_ok[10];
   uint64_t s_full[2], p_full[2], o_full[2];
   uint64_t exchange;  // the softmax warps' barrier (bounded, unlike bar.sync)
   uint32_t tmem_base;
@@ -150,7 +153,8 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       ptx::mbar_init(&sm.q_full, 1);
       ptx::mbar_init(&sm.q_empty, 1);
       for (int i = 0; i < kStages; ++i) {
-        ptx::mbar_init(&sm.kv_full[i], 1);
+        ptx::mbar_init(&sm.k_full[i], 1);
+        ptx::mbar_init(&sm.v_full[i], 1);
         ptx::mbar_init(&sm.kv_empty[i], 1);
         ptx::mbar_init(&sm.v_ok[i], 2);
       }
@@ -327,25 +331,27 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           uint32_t o[32];
           ptx::tmem_ld_32x32b_x32(o_col + c, o);
           ptx::tmem_ld_wait();
-          if (!valid) continue;
-          float v[32];
+          if (valid) {
+            float v[32];
 #pragma unroll
-          for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(o[k]);
-          if (fix) {
+            for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(o[k]);
+            if (fix) {
 #pragma unroll
-            for (int k = 0; k < 32; ++k) v[k] += guard_term(special[c + k], pos - base);
+              for (int k = 0; k < 32; ++k) v[k] += guard_term(special[c + k], pos - base);
+            }
+            if (it.n_splits > 1) {
+#pragma unroll
+              for (int k = 0; k < 32; k += 4)
+                *reinterpret_cast<float4*>(a.part_o + pr * D + c + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 32; k += 8)
+                *reinterpret_cast<uint4*>(dst + c + k) =
+                    make_uint4(f2_to_h2(v[k] * inv, v[k + 1] * inv), f2_to_h2(v[k + 2] * inv, v[k + 3] * inv),
+                               f2_to_h2(v[k + 4] * inv, v[k + 5] * inv), f2_to_h2(v[k + 6] * inv, v[k + 7] * inv));
+            }
           }
-          if (it.n_splits > 1) {
-#pragma unroll
-            for (int k = 0; k < 32; k += 4)
-              *reinterpret_cast<float4*>(a.part_o + pr * D + c + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
-          } else {
-#pragma unroll
-            for (int k = 0; k < 32; k += 8)
-              *reinterpret_cast<uint4*>(dst + c + k) =
-                  make_uint4(f2_to_h2(v[k] * inv, v[k + 1] * inv), f2_to_h2(v[k + 2] * inv, v[k + 3] * inv),
-                             f2_to_h2(v[k + 4] * inv, v[k + 5] * inv), f2_to_h2(v[k + 6] * inv, v[k + 7] * inv));
-          }
+          __syncwarp();  // the next load needs the whole warp
         }
         if (it.n_splits > 1 && valid) a.part_ml[pr] = make_float2(m == -INFINITY ? m : m * scale, l);
       } else {
@@ -381,28 +387,30 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           ptx::tmem_ld_32x32b_x32(lanes + 2 * kTile + c, o0);
           if (n > 1) ptx::tmem_ld_32x32b_x32(lanes + 2 * kTile + D + c, o1);
           ptx::tmem_ld_wait();
-          if (!valid) continue;
-          float v[32];
+          if (valid) {
+            float v[32];
 #pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            v[k] = __uint_as_float(o0[k]) * f0;
-            if (n > 1) v[k] = fmaf(__uint_as_float(o1[k]), f1, v[k]);
+            for (int k = 0; k < 32; ++k) {
+              v[k] = __uint_as_float(o0[k]) * f0;
+              if (n > 1) v[k] = fmaf(__uint_as_float(o1[k]), f1, v[k]);
+            }
+            if (fix) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) v[k] += guard_term(special[c + k], pos - base);
+            }
+            if (it.n_splits > 1) {
+#pragma unroll
+              for (int k = 0; k < 32; k += 4)
+                *reinterpret_cast<float4*>(a.part_o + pr * D + c + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 32; k += 8)
+                *reinterpret_cast<uint4*>(dst + c + k) =
+                    make_uint4(f2_to_h2(v[k] * inv, v[k + 1] * inv), f2_to_h2(v[k + 2] * inv, v[k + 3] * inv),
+                               f2_to_h2(v[k + 4] * inv, v[k + 5] * inv), f2_to_h2(v[k + 6] * inv, v[k + 7] * inv));
+            }
           }
-          if (fix) {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) v[k] += guard_term(special[c + k], pos - base);
-          }
-          if (it.n_splits > 1) {
-#pragma unroll
-            for (int k = 0; k < 32; k += 4)
-              *reinterpret_cast<float4*>(a.part_o + pr * D + c + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
-          } else {
-#pragma unroll
-            for (int k = 0; k < 32; k += 8)
-              *reinterpret_cast<uint4*>(dst + c + k) =
-                  make_uint4(f2_to_h2(v[k] * inv, v[k + 1] * inv), f2_to_h2(v[k + 2] * inv, v[k + 3] * inv),
-                             f2_to_h2(v[k + 4] * inv, v[k + 5] * inv), f2_to_h2(v[k + 6] * inv, v[k + 7] * inv));
-          }
+          __syncwarp();  // the next load needs the whole warp
         }
         if (it.n_splits > 1 && valid && t == 0)
           a.part_ml[pr] = make_float2(m_all == -INFINITY ? m_all : m_all * scale, l_all);
@@ -462,7 +470,14 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         }
         __syncwarp();
       };
-      uint32_t v_phase = 0;  // bit per stage: v_ok completes a phase only when the stage holds a V tile
+      uint32_t k_phase = 0, v_phase = 0;  // a bit per stage: the barriers of a kind only count that kind's tiles
+      auto wait_k = [&]() {
+        const int ks = ring.stage;
+        wait(&sm.k_full[ks], (k_phase >> ks) & 1u, 1);
+        k_phase ^= 1u << ks;
+        advance<kStages>(ring);
+        return ks;
+      };
       auto wait_v = [&]() {
         const int vs = ring.stage;
         wait(&sm.v_ok[vs], (v_phase >> vs) & 1u, 1);
@@ -489,17 +504,15 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         const bool dual = it.n_tok > tile_tokens;
         wait(&sm.q_full, q_phase, 1);
         q_phase ^= 1u;
-        wait(&sm.kv_full[ring.stage], ring.phase, 1);
+        const int first = wait_k();
         ptx::tcgen05_fence_after();
-        issue_qk(0, 0, ring.stage);
-        if (dual) issue_qk(1, 1, ring.stage);
-        commit(&sm.kv_empty[ring.stage]);
-        advance<kStages>(ring);
+        issue_qk(0, 0, first);
+        if (dual) issue_qk(1, 1, first);
+        commit(&sm.kv_empty[first]);
         if (!dual && n > 1) {
-          wait(&sm.kv_full[ring.stage], ring.phase, 1);
-          issue_qk(1, 0, ring.stage);
-          commit(&sm.kv_empty[ring.stage]);
-          advance<kStages>(ring);
+          const int second = wait_k();
+          issue_qk(1, 0, second);
+          commit(&sm.kv_empty[second]);
         }
         if (n <= (dual ? 1 : 2)) commit(&sm.q_empty);
         if (dual) {
@@ -507,10 +520,9 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             const int vs = wait_v();
             wait_p(0);
             issue_pv(0, vs, j > 0);
-            const int ks = ring.stage;
+            int ks = 0;
             if (j + 1 < n) {
-              wait(&sm.kv_full[ks], ring.phase, 1);
-              advance<kStages>(ring);
+              ks = wait_k();
               issue_qk(0, 0, ks);
             } else {
               commit(&sm.o_full[0]);
@@ -534,9 +546,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             issue_pv(t, vs, i > 1);
             commit(&sm.kv_empty[vs]);
             if (i + 2 < n) {
-              const int ks = ring.stage;
-              wait(&sm.kv_full[ks], ring.phase, 1);
-              advance<kStages>(ring);
+              const int ks = wait_k();
               issue_qk(t, 0, ks);
               commit(&sm.kv_empty[ks]);
               if (i + 3 == n) commit(&sm.q_empty);
@@ -582,15 +592,15 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           const int pg = table[first / a.page_size];
           return pg >= 0 && pg < a.num_pages ? pg : a.num_pages;
         };
-        auto load = [&](const CUtensorMap* map, int i, int page) {
+        auto load = [&](const CUtensorMap* map, uint64_t* full, int i, int page) {
           wait(&sm.kv_empty[ring.stage], ring.phase ^ 1u, 0);
           if (!dead) {
-            if (lane == 0) ptx::mbar_arrive_expect_tx(&sm.kv_full[ring.stage], Sh::kTileBytes);
+            if (lane == 0) ptx::mbar_arrive_expect_tx(&full[ring.stage], Sh::kTileBytes);
             __syncwarp();
             if (loads)
               ptx::tma_load_4d(smem + Sh::kRing + ring.stage * Sh::kTileBytes + my_half * Sh::kSubBytes +
                                    my_box * box_tokens * 128,
-                               map, &sm.kv_full[ring.stage], my_half * 64, it.head,
+                               map, &full[ring.stage], my_half * 64, it.head,
                                ((it.tile0 + i) * kTile + my_box * box_tokens) % a.page_size, page);
           }
           __syncwarp();
@@ -604,7 +614,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             bits = ((1u << per_box) - 1u) << (my_box * per_box);
           bits = __reduce_or_sync(0xffffffffu, bits);
           if (lane == 0) sm.valid[(k_count + i) & (kMaskRing - 1)] = bits;
-          load(&map_k, i, page);
+          load(&map_k, sm.k_full, i, page);
         };
         int p0 = page_of(0), p1 = page_of(1), p2;  // pages of the next tiles, read ahead of their use
         // Q: rows (token, head) of this kv head's group
@@ -627,7 +637,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           p2 = 0;
         }
         for (int i = 0; i < n; ++i) {
-          load(&map_v, i, p0);
+          load(&map_v, sm.v_full, i, p0);
           const int next = i + ahead;
           if (ahead == 2) {
             const int p3 = page_of(next + 1);
@@ -654,6 +664,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     } else {
       // =============================== V guard ===============================
       const int part = warp - kGuardWarp;  // this warp's half of the rows
+      uint32_t v_phase = 0;
       Ring ring;
       Item it;
       while (next_item(it, 3)) {
@@ -661,11 +672,11 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         const bool dual = it.n_tok > tile_tokens;
         const int kv_len = it.pos0 + it.n_tok;
         uint32_t* special = sm.special[slot];
-        auto skip_k = [&]() { advance<kStages>(ring); };
-        if (n > 0) skip_k();
-        if (!dual && n > 1) skip_k();
+        if (n > 0) advance<kStages>(ring);  // over the K tiles
+        if (!dual && n > 1) advance<kStages>(ring);
         for (int i = 0; i < n; ++i) {
-          wait(&sm.kv_full[ring.stage], ring.phase, 3);
+          wait(&sm.v_full[ring.stage], (v_phase >> ring.stage) & 1u, 3);
+          v_phase ^= 1u << ring.stage;
           const int t0 = (it.tile0 + i) * kTile;
           uint8_t* tile = smem + Sh::kRing + ring.stage * Sh::kTileBytes;
           // rows behind the context: zeros (whole rows, so the swizzle does not matter)
@@ -692,7 +703,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           __syncwarp();
           if (lane == 0) ptx::mbar_arrive(&sm.v_ok[ring.stage]);
           advance<kStages>(ring);
-          if (i + (dual ? 1 : 2) < n) skip_k();
+          if (i + (dual ? 1 : 2) < n) advance<kStages>(ring);
         }
         release_item();
       }
