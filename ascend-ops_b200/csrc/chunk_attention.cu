@@ -23,47 +23,6 @@ namespace {
 // ---- plan -----------------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024;
 
-struct Seq {
-  int start, n, len, blocks, tiles;  // tiles: kv tiles of the last (longest) block
-};
-
-__device__ __forceinline__ Seq load_seq(const Args& a, int b) {
-  Seq s;
-  const int lo = min(max(a.query_starts[b], 0), a.num_tokens), hi = min(max(a.query_starts[b + 1], 0), a.num_tokens);
-  s.start = lo;
-  s.n = max(hi - lo, 0);
-  s.len = min(max(a.context_lens[b], 0), a.max_pages_per_seq * a.page_size);
-  s.blocks = (s.n + a.block_tokens - 1) / a.block_tokens;
-  s.tiles = (s.len + a.kv_tile - 1) / a.kv_tile;
-  return s;
-}
-
-// Exclusive prefix sum over the block's threads; *total gets the sum.
-__device__ __forceinline__ long long block_prefix(long long v, long long* sums, long long* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long incl = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += u;
-  }
-  __syncthreads();  // `sums` may still be read from the call before
-  if (lane == 31) sums[warp] = incl;
-  __syncthreads();
-  if (warp == 0) {
-    long long x = sums[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += u;
-    }
-    sums[lane] = x;
-  }
-  __syncthreads();
-  *total = sums[31];
-  return incl - v + (warp > 0 ? sums[warp - 1] : 0);
-}
-
 // Per-sequence plan, kept in the workspace behind the prefix array.
 struct SeqPlan {
   int splits, row0, counter0;
@@ -457,8 +416,12 @@ void plan_shape(Args* a, bool tc) {
     a->head_tiles = 1;
     a->block_tokens = 2 * (128 / group);
     a->kv_tile = 128;
-    a->min_tiles = 4;
-    a->target = 2 * sm_count();
+    a->shares = sm_count() < kMaxShares ? sm_count() : kMaxShares;
+    a->slot_rows = (a->block_tokens < a->num_tokens ? a->block_tokens : a->num_tokens) * group;
+    // two records per stretch, unless no context is long enough to be cut
+    const bool cut = a->shares > 1 && static_cast<int64_t>(a->max_pages_per_seq) * a->page_size > 3 * a->kv_tile;
+    a->max_rows = cut ? 2 * a->shares * a->slot_rows : 0;
+    return;
   } else {
     a->group = group < kRows ? group : kRows;
     a->head_tiles = (group + a->group - 1) / a->group;
@@ -491,6 +454,12 @@ size_t lay_out(Args* a, char* base) {
     return p;
   };
   a->header = reinterpret_cast<Header*>(take(sizeof(Header)));
+  if (a->shares > 0) {  // the tcgen05 kernel needs no plan
+    a->cuts = take(a->max_rows > 0 ? cut_list_bytes(a->shares) : 0);
+    a->part_ml = reinterpret_cast<float2*>(take(static_cast<size_t>(a->max_rows) * sizeof(float2)));
+    a->part_o = reinterpret_cast<float*>(take(static_cast<size_t>(a->max_rows) * a->head_dim * sizeof(float)));
+    return off;
+  }
   a->prefix = reinterpret_cast<int*>(take((static_cast<size_t>(a->bs) + 1) * sizeof(int) + static_cast<size_t>(a->bs) * sizeof(SeqPlan)));
   a->counters = reinterpret_cast<int*>(take(static_cast<size_t>(a->max_split_items) * sizeof(int)));
   a->items = reinterpret_cast<Item*>(take(static_cast<size_t>(a->max_items) * sizeof(Item)));
@@ -609,7 +578,7 @@ extern "C" int b200ops_chunked_paged_attention(const void* q, const void* key_ca
   a.layout = layout;
   a.scale_log2 = (1.0f / std::sqrt(static_cast<float>(head_dim))) * 1.44269504088896340736f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (tc) return ca::launch_tc(a, st);
   const int pr = ca::launch_plan(a, st);
-  if (pr != B200OPS_OK) return pr;
-  return tc ? ca::launch_tc(a, st) : ca::launch_general(a, st);
+  return pr != B200OPS_OK ? pr : ca::launch_general(a, st);
 }

@@ -26,6 +26,8 @@ struct Item {
   int pad;
 };
 
+constexpr int kMaxShares = 160;
+
 struct Header {
   int n_items;
   int ticket;  // next item to hand out
@@ -57,9 +59,52 @@ struct Args {
   int min_tiles;     // a split is at least this many kv tiles
   int target;        // items wanted at least
   int max_items, max_split_items, max_rows;
+  // tcgen05 kernel: CTAs, rows of a part's record, the cut units of the call (workspace)
+  int shares, slot_rows;
+  void* cuts;
 };
 
 #ifdef __CUDACC__
+struct Seq {
+  int start, n, len, blocks, tiles;  // first row, new tokens, context, blocks, kv tiles of the last block
+};
+
+__device__ __forceinline__ Seq load_seq(const Args& a, int b) {
+  Seq s;
+  const int lo = min(max(a.query_starts[b], 0), a.num_tokens), hi = min(max(a.query_starts[b + 1], 0), a.num_tokens);
+  s.start = lo;
+  s.n = max(hi - lo, 0);
+  s.len = min(max(a.context_lens[b], 0), a.max_pages_per_seq * a.page_size);
+  s.blocks = (s.n + a.block_tokens - 1) / a.block_tokens;
+  s.tiles = (s.len + a.kv_tile - 1) / a.kv_tile;
+  return s;
+}
+
+// Exclusive prefix sum over the block's threads (whole warps); *total gets the sum.  `sums`: 32 words
+// of shared memory.
+__device__ __forceinline__ long long block_prefix(long long v, long long* sums, long long* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long incl = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += u;
+  }
+  __syncthreads();  // `sums` may still be read from the call before
+  if (lane == 31) sums[warp] = incl;
+  __syncthreads();
+  const int warps = static_cast<int>(blockDim.x) >> 5;
+  long long x = lane < warps ? sums[lane] : 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += u;
+  }
+  *total = __shfl_sync(0xffffffffu, x, 31);
+  const long long before = __shfl_sync(0xffffffffu, x, max(warp - 1, 0));
+  return incl - v + (warp > 0 ? before : 0);
+}
+
 // Non-finite values among hidden keys.  A hidden key's probability is exactly 0, but the matrix
 // product still forms 0 * v, which is NaN if v is infinite or NaN.  So the kernels take such values
 // out of the V tiles at positions that some row of the block does not see, remember per channel the
@@ -108,6 +153,7 @@ int launch_plan(const Args& a, cudaStream_t st);
 int launch_general(const Args& a, cudaStream_t st);
 bool tc_supported(int64_t head_dim, int64_t group, int64_t page_size, int layout);
 int launch_tc(const Args& a, cudaStream_t st);
+size_t cut_list_bytes(int shares);
 
 }  // namespace ca
 }  // namespace b200ops

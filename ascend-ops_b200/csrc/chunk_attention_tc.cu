@@ -1,16 +1,17 @@
 // Attention of chunks of new tokens over the paged KV cache on the 5th-generation tensor cores:
 // head_dim 64 or 128, caches [pages, P, Hkv, D] with P a multiple of 8, up to 128 query heads per kv head.
 //
-// One persistent CTA per SM draws items (chunk_attention.cuh) and works on two 128-row score tiles
-// at a time:  S_t = Q_t K^T and O_t += P_t V, t = 0, 1, both accumulators in TMEM (2 x 128 columns for
+// One persistent CTA per SM takes an equal share of the batch's work (below) and computes two 128-row
+// score tiles at a time:  S_t = Q_t K^T and O_t += P_t V, t = 0, 1, both accumulators in TMEM (2 x 128 columns for
 // S, 2 x D for O; P_t is written back over S_t as fp16 and read from TMEM as the second product's left
 // operand).  While the tensor core works on one tile, a warpgroup takes the exponentials of the
 // other.  The two tiles are
 //   - the two halves of a block of more than 128 rows: both read the same K and V tile; or
 //   - for a block of at most 128 rows (decoding, short chunks): the even and the odd kv tiles of its range,
 //     two running softmaxes that are merged at the end.
-// Roles: warps 0-3 and 4-7 softmax of tile 0 and 1 (a thread owns a row), warp 8 issues the MMAs,
-// warp 9 walks the block table and issues the TMA loads, warps 10-11 guard the V tiles (below).
+// Roles: warps 0-3 and 4-7 softmax of tile 0 and 1 (a thread owns a row), warps 8 and 9
+// issue the MMAs of tile 0 and 1, warp 10 walks the block table and issues the TMA loads, warp 11 guards
+// the V tiles (below).
 //
 // Online softmax: a row's reference maximum is only raised when the new maximum exceeds it by more
 // than 2^8 in the exponential, so the accumulator in TMEM is rescaled a few times per item instead of
@@ -18,7 +19,7 @@
 // by the sum in fp32 makes up for any reference.
 //
 // V tiles: a hidden key has probability 0, but 0 * inf is NaN.  Slots past the context and pages that
-// name nothing are filled with zeros (by TMA outside the tensor, by the guard warps inside a box), and
+// name nothing are filled with zeros (by TMA outside the tensor, by the guard warp inside a box), and
 // the non-finite values of keys that some row of the block does not see are taken out and
 // accounted for at the end (take_nonfinite).
 #include "chunk_attention.cuh"
@@ -33,38 +34,198 @@ namespace {
 
 constexpr int kThreads = 384;
 constexpr int kTile = 128;  // keys per kv tile, rows per score tile
+constexpr int kHalf = 64;   // keys per score buffer
 constexpr int kMaskRing = 16;
-constexpr int kMmaWarp = 8, kProducerWarp = 9, kGuardWarp = 10;
+constexpr int kMmaWarp = 8, kProducerWarp = 10, kGuardWarp = 11;  // MMA: 8 and 9, one per score tile
 constexpr uint32_t kSoftmaxWarps = 8;
 constexpr int kErrBase = 21;  // 21 producer, 22 MMA, 23 softmax, 24 guard, 25 misaligned shared memory
 
 __device__ int g_ca_status = 0;
+
+// ---- shares of the work -------------------------------------------------------------------
+// The batch is a line of units (sequence, kv head, block of tokens), each as long as the keys its
+// last token sees plus a constant for its start and end; CTA c of S takes the stretch
+// [c, c + 1) * total / S.  Every CTA finds its stretch from the lengths by itself (one pass over the
+// sequences, arithmetic inside one), so there is no planning launch and no ticket counter.  A unit
+// that a stretch boundary falls into is cut there, at a whole kv tile.  So at most S - 1 units are cut
+// whatever the batch, and all CTAs finish together.  The parts of a cut unit are written un-normalised
+// and merged by a second launch, which spreads the rows over all SMs (the last part's CTA merging alone
+// was measured too: 5 us more per prefill, and far slower where one unit has dozens of parts).
+constexpr int kOverheadTokens = 256;
+
+struct Line {
+  long long total, share;
+};
+
+__device__ __forceinline__ long long unit_base(const Seq& s) { return max(s.len - s.n, 0) + kOverheadTokens; }
+// A block of more than one score tile takes twice the time per key (measured 2.3 us and 1.2 us per kv
+// tile); only the last block of a sequence can be the smaller kind.
+__device__ __forceinline__ int unit_weight(const Args& a, const Seq& s, int block) {
+  return s.n - block * a.block_tokens > a.block_tokens / 2 ? 2 : 1;
+}
+__device__ __forceinline__ long long unit_length(const Args& a, const Seq& s, int block) {
+  return unit_weight(a, s, block) * (unit_base(s) + static_cast<long long>(a.block_tokens) * (block + 1));
+}
+// Length of the first m blocks of one head.
+__device__ __forceinline__ long long blocks_length(const Args& a, const Seq& s, long long m) {
+  if (m <= 0) return 0;
+  const long long k = m - 1;  // blocks of two tiles, then one of either kind
+  return 2 * (k * unit_base(s) + a.block_tokens * (k * (k + 1) / 2)) + unit_length(a, s, static_cast<int>(k));
+}
+
+struct Unit {
+  Seq s;
+  int seq, head, block;
+  long long at;  // where it starts on the line
+  int n_tok, pos0, tiles;
+  long long length;
+};
+
+__device__ __forceinline__ void set_block(const Args& a, Unit& u) {
+  u.n_tok = min(a.block_tokens, u.s.n - u.block * a.block_tokens);
+  u.pos0 = u.s.len - u.s.n + u.block * a.block_tokens;
+  u.tiles = (max(u.pos0 + u.n_tok, 0) + a.kv_tile - 1) / a.kv_tile;
+  u.length = unit_length(a, u.s, u.block);
+}
+
+// Tile at which a boundary `x` behind the unit's start cuts it; 0 or `tiles`: it does not.
+__device__ __forceinline__ int cut_tile(const Unit& u, long long x, long long share) {
+  if (x <= 0) return 0;
+  if (x >= u.length) return u.tiles;
+  // Short shares (small batches): parts of four tiles, or the merge costs more than the parts save.
+  const int grain = share >= 4096 ? 1 : 4, least = share >= 4096 ? 2 : 4;
+  // fp32 with each operation rounded by itself: cheaper than a 64-bit division, the same in both
+  // kernels, and it never decreases in x
+  int k = min(static_cast<int>(__fdiv_rn(__fmul_rn(static_cast<float>(x), static_cast<float>(u.tiles)),
+                                         static_cast<float>(u.length))), u.tiles);
+  k -= k % grain;
+  return k < least ? 0 : (u.tiles - k < least ? u.tiles : k);
+}
+
+struct Found {
+  int seq;
+  long long at;
+};
+
+// Whole block: the line, and the sequence that holds position index * share (left in *found by the
+// thread that meets it; seq = bs if the position lies behind the end).
+__device__ __forceinline__ Line find_share(const Args& a, int shares, long long index, long long* sums, Found* found) {
+  const int run = (a.bs + static_cast<int>(blockDim.x) - 1) / static_cast<int>(blockDim.x);
+  const int b0 = min(static_cast<int>(threadIdx.x) * run, a.bs), b1 = min(b0 + run, a.bs);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    const Seq s = load_seq(a, b);
+    mine += a.num_kv_heads * blocks_length(a, s, s.blocks);
+  }
+  if (threadIdx.x == 0) found->seq = a.bs;
+  Line line;
+  long long at = block_prefix(mine, sums, &line.total);
+  line.share = max((line.total + shares - 1) / shares, 1LL);
+  const long long x = index * line.share;
+  if (at <= x && x < at + mine) {
+    for (int b = b0; b < b1; ++b) {
+      const Seq s = load_seq(a, b);
+      const long long len = a.num_kv_heads * blocks_length(a, s, s.blocks);
+      if (x < at + len) {
+        found->seq = b;
+        found->at = at;
+        break;
+      }
+      at += len;
+    }
+  }
+  __syncthreads();
+  return line;
+}
+
+// The unit that holds position x of the line, inside sequence f.seq.
+__device__ __forceinline__ Unit unit_at(const Args& a, const Found& f, long long x) {
+  Unit u;
+  u.seq = f.seq;
+  u.s = load_seq(a, f.seq);
+  const long long per_head = blocks_length(a, u.s, u.s.blocks);
+  u.head = min(static_cast<int>(static_cast<float>(x - f.at) / static_cast<float>(per_head)), a.num_kv_heads - 1);
+  long long y = x - f.at - u.head * per_head;
+  while (y < 0) y += per_head, --u.head;  // the quotient was rounded
+  while (y >= per_head) y -= per_head, ++u.head;
+  int lo = 0, hi = u.s.blocks;  // the last block that starts at or before y
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (blocks_length(a, u.s, mid) <= y) lo = mid; else hi = mid;
+  }
+  u.block = lo;
+  u.at = f.at + u.head * per_head + blocks_length(a, u.s, lo);
+  set_block(a, u);
+  return u;
+}
+
+// The next unit of the line; false behind the last.
+__device__ __forceinline__ bool next_unit(const Args& a, Unit& u) {
+  u.at += u.length;
+  if (++u.block == u.s.blocks) {
+    u.block = 0;
+    if (++u.head == a.num_kv_heads) {
+      u.head = 0;
+      do {
+        if (++u.seq >= a.bs) return false;
+        u.s = load_seq(a, u.seq);
+      } while (u.s.blocks == 0);
+    }
+  }
+  set_block(a, u);
+  return true;
+}
+
+// What the CTA's roles are told of a unit or its part.
+struct Work {
+  int q_tok, n_tok, pos0, seq, head;
+  int tile0, tile1;
+  int part;  // record to write (see part_of); -1: the unit is whole, write the result
+};
+
+// Whether the second half of the last kv tile lies behind every key that the block sees.
+__device__ __forceinline__ bool half_empty(const Work& w) {
+  return w.pos0 + w.n_tok - (w.tile1 - 1) * kTile <= kHalf;
+}
+
+// A cut unit, as the merge needs it; left by the CTA that has its first part (n = 0: none).
+struct CutUnit {
+  int n, q_tok, n_tok, head;
+  int parts[kMaxShares];
+};
+
+// Record of the part of a cut unit that CTA c has: 2 c + 1 for the unit's first part (the end of c's
+// stretch), else 2 c (its start); -1: c has none.
+__device__ __forceinline__ int part_of(const Unit& u, int c, long long share) {
+  const int lo = cut_tile(u, c * share - u.at, share), hi = cut_tile(u, (c + 1) * share - u.at, share);
+  return lo >= hi ? -1 : (lo > 0 ? 2 * c : 2 * c + 1);
+}
 
 template <int D>
 struct Shape {
   static constexpr int kHalves = D / 64;                    // 64-channel sub-tiles
   static constexpr int kSubBytes = kTile * 128;             // [128 rows][64 halfs]
   static constexpr int kTileBytes = kHalves * kSubBytes;    // one Q, K or V tile
-  static constexpr int kStages = D == 128 ? 5 : 10;
+  static constexpr int kPairBytes = 2 * kTileBytes;         // a V tile, then the K tile that goes with it
+  static constexpr int kStages = D == 128 ? 2 : 4;          // pairs in the ring, a power of two
   static constexpr int kQ = 0;
   static constexpr int kRing = 2 * kTileBytes;
-  static constexpr int kMeta = kRing + kStages * kTileBytes;
+  static constexpr int kMeta = kRing + kStages * kPairBytes;
 };
 
 struct Meta {
   uint64_t item_full[2], item_empty[2];
   uint64_t q_full, q_empty;
-  // A stage holds a K or a V tile in turn.  Each kind has arrival barriers of its own, because the guard
-  // warps follow the V tiles alone and a copy may land long after ones issued behind it: with one
-  // barrier per stage they could take the tile before theirs for theirs.
-  uint64_t k_full[10], v_full[10], kv_empty[10], v_ok[10];
-  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t pair_full[4], pair_ok[4], pair_empty[4];  // landed; looked over by the guard; used up
+  uint64_t s_full[2][2], p_full[2][2];  // [score tile][half of the keys]
+  uint64_t pv_done[2], o_full[2];        // after an item's last but one and last second product
   uint64_t exchange;  // the softmax warps' barrier (bounded, unlike bar.sync)
   uint32_t tmem_base;
   int abort_flag;
-  int last;
   int special_flag[2];
-  Item items[2];
+  Work items[2];
+  Found found;
+  long long sums[32];
   uint32_t valid[kMaskRing];     // per kv tile: bit i = keys 8i .. 8i+7 lie in a page that exists
   float swap[2][kTile];          // per tile and row: maxima, then sums, of a block of one score tile
   uint32_t special[2][128];      // per item slot and channel: packed positions, see guard
@@ -74,23 +235,64 @@ template <int D>
 constexpr size_t smem_bytes() { return Shape<D>::kMeta + sizeof(Meta); }
 static_assert(smem_bytes<128>() <= 232448 && smem_bytes<64>() <= 232448, "shared memory");
 
-struct Ring {
-  int stage = 0;
-  uint32_t phase = 0;
-};
-template <int kStages>
-__device__ __forceinline__ void advance(Ring& r) {
-  if (++r.stage == kStages) {
-    r.stage = 0;
-    r.phase ^= 1u;
-  }
-}
-
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// Pairs of floats in one 64-bit register: one instruction for both.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ void split(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float v;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
+  return v;
+}
+
+// 2^x of a pair without the special-function unit, for x <= 64: x = n + f with |f| <= 1/2 (adding
+// 1.5 * 2^23 rounds to an integer in the low mantissa bits), a polynomial of degree 4 in f (relative
+// minimax on [-1/2, 1/2]: 2.6e-6, a hundredth of the fp16 rounding that follows), n added to the
+// exponent.  Below -126 the result stays near 2^-126, which rounds to 0.  NaN and inf: the caller's.
+__device__ __forceinline__ void ex2_poly(uint64_t x2, float& ya, float& yb) {
+  constexpr float kRound = 12582912.f;
+  float xa, xb;
+  split(x2, xa, xb);
+  x2 = pair(fmaxf(xa, -126.f), fmaxf(xb, -126.f));
+  const uint64_t t2 = add2(x2, pair(kRound, kRound));
+  const uint64_t n2 = add2(t2, pair(-kRound, -kRound));
+  const uint64_t f2 = fma2(n2, pair(-1.f, -1.f), x2);
+  uint64_t p2 = pair(0.009570102207362652f, 0.009570102207362652f);
+  p2 = fma2(p2, f2, pair(0.05591785907745361f, 0.05591785907745361f));
+  p2 = fma2(p2, f2, pair(0.240247443318367f, 0.240247443318367f));
+  p2 = fma2(p2, f2, pair(0.6931217908859253f, 0.6931217908859253f));
+  p2 = fma2(p2, f2, pair(0.9999992847442627f, 0.9999992847442627f));
+  float ta, tb;
+  split(t2, ta, tb);
+  split(p2, ya, yb);
+  ya = __uint_as_float((__float_as_uint(ta) << 23) + __float_as_uint(ya));
+  yb = __uint_as_float((__float_as_uint(tb) << 23) + __float_as_uint(yb));
+}
+
+// Of every 8 pairs of exponentials this many are taken by the polynomial: the special-function unit alone
+// needs as long for a score tile as the tensor core for both products.
+constexpr int kPolyPairs = 0;
 
 // Special positions of one channel: three 10-bit fields (+inf, -inf, NaN), the first position
 // minus `base`, 1023 = never.  base = the block's first hidden position, and a block spans at most
@@ -125,6 +327,37 @@ __device__ __forceinline__ float guard_term(uint32_t special, int seen) {
   return s;
 }
 
+// 32 channels of a row.  A thread owns a row, so the lanes of a store lie a row apart: whole 32-byte
+// sectors per lane keep the number of store instructions and the traffic to L2 down (16-byte stores
+// took 3 us per block).
+__device__ __forceinline__ void store_part(float* p, const float (&v)[32]) {
+#pragma unroll
+  for (int k = 0; k < 32; k += 8) {
+    Vec256 w;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w.r[i] = __float_as_uint(v[k + i]);
+    st256(p + k, w);
+  }
+}
+
+__device__ __forceinline__ void store_row(__half* p, const float (&v)[32], float f, bool wide) {
+  uint32_t h[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) h[k] = f2_to_h2(v[2 * k] * f, v[2 * k + 1] * f);
+  if (wide) {
+#pragma unroll
+    for (int k = 0; k < 16; k += 8) {
+      Vec256 w;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w.r[i] = h[k + i];
+      st256(p + 2 * k, w);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 16; k += 4) *reinterpret_cast<uint4*>(p + 2 * k) = make_uint4(h[k], h[k + 1], h[k + 2], h[k + 3]);
+  }
+}
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
 chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -144,19 +377,21 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
         ptx::mbar_init(&sm.item_full[i], 1);
-        ptx::mbar_init(&sm.item_empty[i], kSoftmaxWarps + 3);
-        ptx::mbar_init(&sm.s_full[i], 1);
-        ptx::mbar_init(&sm.p_full[i], 4);
+        ptx::mbar_init(&sm.item_empty[i], kSoftmaxWarps + 3);  // and two MMA warps, the guard
+        for (int b = 0; b < 2; ++b) {
+          ptx::mbar_init(&sm.s_full[i][b], 1);
+          ptx::mbar_init(&sm.p_full[i][b], 4);
+        }
+        ptx::mbar_init(&sm.pv_done[i], 1);
         ptx::mbar_init(&sm.o_full[i], 1);
         sm.special_flag[i] = 0;
       }
       ptx::mbar_init(&sm.q_full, 1);
-      ptx::mbar_init(&sm.q_empty, 1);
+      ptx::mbar_init(&sm.q_empty, 2);
       for (int i = 0; i < kStages; ++i) {
-        ptx::mbar_init(&sm.k_full[i], 1);
-        ptx::mbar_init(&sm.v_full[i], 1);
-        ptx::mbar_init(&sm.kv_empty[i], 1);
-        ptx::mbar_init(&sm.v_ok[i], 2);
+        ptx::mbar_init(&sm.pair_full[i], 1);
+        ptx::mbar_init(&sm.pair_ok[i], 1);
+        ptx::mbar_init(&sm.pair_empty[i], 2);
       }
       ptx::mbar_init(&sm.exchange, kSoftmaxWarps);
       sm.abort_flag = 0;
@@ -177,26 +412,34 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   ptx::tcgen05_fence_after();
   pdl_wait();
   const uint32_t tmem = sm.tmem_base;
+  const Line line = find_share(a, gridDim.x, blockIdx.x, sm.sums, &sm.found);
 
   const int group = a.group;
   const int tile_tokens = a.block_tokens / 2;  // tokens per score tile
+  const int slot_rows = a.slot_rows;
 
   // A wait that runs out (a broken pipeline) is recorded and every later wait of the CTA gives up
   // at once, so that all roles run through to the end.
   bool dead = false;
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
     if (dead) return;
-    if (!__all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, &sm.abort_flag))) {  // the warp stays together
+    if (!ptx::mbar_wait(bar, parity, &sm.abort_flag)) {
       dead = true;
       *reinterpret_cast<volatile int*>(&sm.abort_flag) = 1;
       atomicCAS(&g_ca_status, 0, kErrBase + code);
     }
   };
 
+  // Pair p of an item: K tile p and V tile p - ahead, the two that one step of the MMA loop reads (the
+  // first `ahead` pairs have no V, the last ones no K).  Pair number c of the CTA lies in stage
+  // c mod kStages.
+  auto stage_of = [](uint32_t c) { return c & (kStages - 1); };
+  auto phase_of = [](uint32_t c) { return (c / kStages) & 1u; };
+
   // Items arrive through a two-slot ring.
   int slot = 0;
   uint32_t slot_phase = 0;
-  auto next_item = [&](Item& it, int code) {
+  auto next_item = [&](Work& it, int code) {
     wait(&sm.item_full[slot], slot_phase, code);
     it = sm.items[slot];
     return !dead && it.n_tok > 0;
@@ -210,16 +453,18 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 
   if (warp < static_cast<int>(kSoftmaxWarps)) {
     // =============================== softmax ===============================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     const int t = warp >> 2;                    // score tile
     const int row = (warp & 3) * 32 + lane;     // row of the tile = TMEM lane
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t s_col = lanes + t * kTile;
     const uint32_t o_col = lanes + 2 * kTile + t * D;
-    uint32_t s_phase = 0, o_phase = 0, x_phase = 0, o_other = 0;
+    uint32_t s_phase = 0, o_phase = 0, x_phase = 0, o_other = 0;  // s_phase: a bit per half
+    uint32_t pv_phase = 0;
     uint32_t k_count = 0;  // kv tiles before this item
     const int tok = row / group, head = row - tok * group;
     const float scale = a.scale_log2;
+    const bool wide = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0;
     auto exchange = [&]() {
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&sm.exchange);
@@ -227,7 +472,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       x_phase ^= 1u;
     };
 
-    Item it;
+    Work it;
     while (next_item(it, 2)) {
       const int n = it.tile1 - it.tile0;
       const bool dual = it.n_tok > tile_tokens;
@@ -242,195 +487,217 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         release_item();
         continue;
       }
+      // Halves of kv tiles that this warpgroup sees; the last tile's second half may hold no key at all.
       const int my_n = dual ? n : (n + 1 - t) / 2;
+      const int halves = 2 * my_n - (half_empty(it) && (dual || t == ((n - 1) & 1)) ? 1 : 0);
       float m = -INFINITY, l = 0.f;  // reference maximum (raw scores) and sum
-      for (int j = 0; j < my_n; ++j) {
-        const int idx = dual ? j : 2 * j + t;
-        const int last_col = pos - (it.tile0 + idx) * kTile;  // last visible key of the tile
-        wait(&sm.s_full[t], s_phase, 2);
-        s_phase ^= 1u;
+      float limit = -INFINITY;       // scores up to here keep the reference
+      const int row_pos = pos - it.tile0 * kTile;               // this row's position behind the first key
+      const int warp_pos = __shfl_sync(0xffffffffu, row_pos, 0);  // the least of the warp's
+      int off = dual ? 0 : t * kTile;                           // first key of the half
+      auto await_scores = [&](int b) {
+        wait(&sm.s_full[t][b], (s_phase >> b) & 1u, 2);
+        s_phase ^= 1u << b;
         ptx::tcgen05_fence_after();
-        uint32_t s[4][32];
+      };
+      auto load_scores = [&](int b, uint32_t (&s)[2][32]) {
+        ptx::tmem_ld_32x32b_x32(s_col + b * kHalf, s[0]);
+        ptx::tmem_ld_32x32b_x32(s_col + b * kHalf + 32, s[1]);
+      };
+      // Half i of the keys, whose scores are in s; leaves those of the next half there.
+      auto step = [&](int i, uint32_t (&s)[2][32]) {
+        const int b = i & 1;
+        const uint32_t ok = (sm.valid[(k_count + (off >> 7)) & (kMaskRing - 1)] >> (8 * b)) & 0xffu;
+        if (ok != 0xffu || warp_pos - off < kHalf - 1) {
+          const int last_col = row_pos - off;  // last visible key of the half
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ptx::tmem_ld_32x32b_x32(s_col + i * 32, s[i]);
-        const uint32_t ok = sm.valid[(k_count + idx) & (kMaskRing - 1)];
-        ptx::tmem_ld_wait();
-        if (ok != 0xffffu || __any_sync(0xffffffffu, last_col < kTile - 1)) {
+          for (int g = 0; g < 2; ++g) {
+            const int vis = min(max(last_col + 1 - g * 32, 0), 32);
+            // a bit per column: visible by position, and its group of eight keys in a page that exists
+            const uint32_t bits = (vis == 32 ? 0xffffffffu : (1u << vis) - 1u) &
+                                  ((((ok >> (4 * g)) & 15u) * 0x00204081u & 0x01010101u) * 0xffu);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              const int col = i * 32 + c;
-              if (col > last_col || !((ok >> (col >> 3)) & 1u)) s[i][c] = __float_as_uint(-INFINITY);
-            }
-        }
-        float mx[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          mx[i] = __uint_as_float(s[i][0]);
-#pragma unroll
-          for (int c = 1; c < 32; ++c) mx[i] = fmaxf(mx[i], __uint_as_float(s[i][c]));
-        }
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        const bool raise = top > m && (m == -INFINITY || (top - m) * scale > 8.f);
-        if (__any_sync(0xffffffffu, raise)) {
-          const float f = raise ? ex2((m - top) * scale) : 1.f;  // m = -inf: 0
-          if (raise) m = top;
-          l *= f;
-          if (j > 0) {
-#pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              ptx::tmem_ld_32x32b_x32(o_col + c, o);
-              ptx::tmem_ld_wait();
-#pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-              ptx::tmem_st_32x32b_x32(o_col + c, o);
-            }
+            for (int c = 0; c < 32; ++c)
+              if (!((bits >> c) & 1u)) s[g][c] = __float_as_uint(-INFINITY);
           }
         }
-        const float shift = m == -INFINITY ? 0.f : -m * scale;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        off += b == 0 || dual ? kHalf : 2 * kTile - kHalf;
+        uint32_t p[32];
+        const uint64_t scale2 = pair(scale, scale);
+        uint64_t sum2[2];
+        auto exponentials = [&](int from, int to) {
+          const float shift = m == -INFINITY ? 0.f : -m * scale;
+          const uint64_t shift2 = pair(shift, shift);
+          if (from == 0) sum2[0] = sum2[1] = 0;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t p[32];
-#pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            const int i = 2 * h + (c >> 4), k = 2 * (c & 15);
-            const float p0 = ex2(fmaf(__uint_as_float(s[i][k]), scale, shift));
-            const float p1 = ex2(fmaf(__uint_as_float(s[i][k + 1]), scale, shift));
-            sum[c & 1] += p0;
-            sum[2 + (c & 1)] += p1;
+          for (int c = from; c < to; ++c) {
+            const int g = c >> 4, k = 2 * (c & 15);
+            const uint64_t x2 = fma2(pair(__uint_as_float(s[g][k]), __uint_as_float(s[g][k + 1])), scale2, shift2);
+            float p0, p1;
+            if ((c & 7) < kPolyPairs) {
+              ex2_poly(x2, p0, p1);
+            } else {
+              split(x2, p0, p1);
+              p0 = ex2(p0);
+              p1 = ex2(p1);
+            }
+            sum2[c & 1] = add2(sum2[c & 1], pair(p0, p1));
             p[c] = f2_to_h2(p0, p1);
           }
-          ptx::tmem_st_32x32b_x32(s_col + h * 32, p);
+        };
+        // The reference maximum is nearly always still good: the first exponentials are taken with it while
+        // the half's own maximum is being found, and again in the rare case that it was not.
+        exponentials(0, 16);
+        float mx[2];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          mx[g] = __uint_as_float(s[g][0]);
+#pragma unroll
+          for (int c = 2; c < 32; c += 2) mx[g] = max3_nan(mx[g], __uint_as_float(s[g][c]), __uint_as_float(s[g][c - 1]));
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        const float top = max3_nan(max3_nan(mx[0], mx[1], __uint_as_float(s[0][31])), __uint_as_float(s[1][31]), mx[0]);
+        if (__any_sync(0xffffffffu, !(top <= limit))) {
+          float f = 1.f;
+          if (!(top < INFINITY)) {
+            l = NAN;  // a visible score is +inf or NaN: so is the softmax
+          } else if (top > limit) {
+            f = ex2((m - top) * scale);  // from -inf: 0
+            m = top;
+            limit = top + 8.f / scale;
+            l *= f;
+          }
+          if (i > 0) {
+            // The accumulator follows, once the product before this one is in it: the next half's scores are
+            // computed behind that product; behind the last half, its own barrier tells.
+            if (i + 1 < halves)
+              wait(&sm.s_full[t][b ^ 1], (s_phase >> (b ^ 1)) & 1u, 2);
+            else
+              wait(&sm.pv_done[t], pv_phase, 2);
+            ptx::tcgen05_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D; c += 8) {  // a few columns at a time: the scores stay in registers
+              uint32_t o[8];
+              ptx::tmem_ld_32x32b_x8(o_col + c, o);
+              ptx::tmem_ld_wait();
+#pragma unroll
+              for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              ptx::tmem_st_32x32b_x8(o_col + c, o);
+            }
+          }
+          exponentials(0, 16);
+        }
+        exponentials(16, 32);
+        float x, y;
+        split(add2(sum2[0], sum2[1]), x, y);
+        l += x + y;
+        // The next scores are on their way while the probabilities are stored (they were issued behind the
+        // product before this half's, so waiting for them first holds nothing up).
+        if (i + 1 < halves) {
+          await_scores(b ^ 1);
+          load_scores(b ^ 1, s);
+        }
+        ptx::tmem_st_32x32b_x32(s_col + b * kHalf, p);
         ptx::tmem_st_wait();
         ptx::tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&sm.p_full[t]);
+        if (lane == 0) ptx::mbar_arrive(&sm.p_full[t][b]);
+        ptx::tmem_ld_wait();
+      };
+      if (!__any_sync(0xffffffffu, valid)) {  // no row of this warp is anybody's: its P may be anything
+        for (int i = 0; i < halves; ++i) {
+          await_scores(i & 1);
+          if (lane == 0) ptx::mbar_arrive(&sm.p_full[t][i & 1]);
+        }
+      } else if (halves > 0) {
+        uint32_t s[2][32];
+        await_scores(0);
+        load_scores(0, s);
+        ptx::tmem_ld_wait();
+#pragma unroll 1
+        for (int i = 0; i < halves; ++i) step(i, s);
       }
+      if (halves > 1) pv_phase ^= 1u;
       k_count += n;
 
       // ------------------------------ the item's result ------------------------------
-      const int rows = it.n_tok * group;
       const int base = it.pos0 + 1;  // first hidden position of the block
       uint32_t* special = sm.special[slot];
-      bool fix;  // some value was taken out of this item's V tiles
+      // The row's sums are f0 * O_0 + f1 * O_1 over channels [c0, c1): of a block of two score tiles its own
+      // accumulator; else the even and the odd kv tiles' accumulators (a warp may read its 32 lanes of
+      // either), each warpgroup taking half of the channels after both learned both maxima and sums.
+      float f0 = 1.f, f1 = 0.f;
+      uint32_t col0 = o_col, col1 = 0;
+      int c0 = 0, c1 = D;
+      bool both = false;
       if (dual) {
         wait(&sm.o_full[t], o_phase, 2);
         o_phase ^= 1u;
         o_other ^= 1u;
-        ptx::tcgen05_fence_after();
-        fix = *reinterpret_cast<volatile int*>(&sm.special_flag[slot]) != 0;
-        const float inv = it.n_splits > 1 ? 1.f : (l == 0.f ? 0.f : 1.0f / l);
-        const size_t pr = static_cast<size_t>(it.row0) + static_cast<size_t>(it.split) * rows + my_tok * group + head;
-#pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          ptx::tmem_ld_32x32b_x32(o_col + c, o);
-          ptx::tmem_ld_wait();
-          if (valid) {
-            float v[32];
-#pragma unroll
-            for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(o[k]);
-            if (fix) {
-#pragma unroll
-              for (int k = 0; k < 32; ++k) v[k] += guard_term(special[c + k], pos - base);
-            }
-            if (it.n_splits > 1) {
-#pragma unroll
-              for (int k = 0; k < 32; k += 4)
-                *reinterpret_cast<float4*>(a.part_o + pr * D + c + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
-            } else {
-#pragma unroll
-              for (int k = 0; k < 32; k += 8)
-                *reinterpret_cast<uint4*>(dst + c + k) =
-                    make_uint4(f2_to_h2(v[k] * inv, v[k + 1] * inv), f2_to_h2(v[k + 2] * inv, v[k + 3] * inv),
-                               f2_to_h2(v[k + 4] * inv, v[k + 5] * inv), f2_to_h2(v[k + 6] * inv, v[k + 7] * inv));
-            }
-          }
-          __syncwarp();  // the next load needs the whole warp
-        }
-        if (it.n_splits > 1 && valid) a.part_ml[pr] = make_float2(m == -INFINITY ? m : m * scale, l);
       } else {
-        // Even and odd kv tiles: both warpgroups learn both maxima and sums, then each takes half of
-        // the channels of both accumulators (a warp may read its 32 lanes of either).
-        sm.swap[t][row] = my_n > 0 ? m : -INFINITY;
+        sm.swap[t][row] = m;
         exchange();
         const float m_other = sm.swap[t ^ 1][row];
         const float m_all = fmaxf(m, m_other);
         const float f = m == -INFINITY ? 0.f : ex2((m - m_all) * scale);
         exchange();
-        sm.swap[t][row] = l * f;
+        l *= f;
+        sm.swap[t][row] = l;
         exchange();
-        const float l_all = l * f + sm.swap[t ^ 1][row];
+        const float l_other = sm.swap[t ^ 1][row];
+        l = t == 0 ? l + l_other : l_other + l;  // the same order on both sides
         const float f_other = m_other == -INFINITY ? 0.f : ex2((m_other - m_all) * scale);
-        const float f0 = t == 0 ? f : f_other, f1 = t == 0 ? f_other : f;
+        m = m_all;
+        f0 = t == 0 ? f : f_other;
+        f1 = t == 0 ? f_other : f;
+        both = n > 1;
         wait(&sm.o_full[0], t == 0 ? o_phase : o_other, 2);
-        if (n > 1) wait(&sm.o_full[1], t == 0 ? o_other : o_phase, 2);
-        if (t == 0) {
-          o_phase ^= 1u;
-          if (n > 1) o_other ^= 1u;
-        } else {
-          o_other ^= 1u;
-          if (n > 1) o_phase ^= 1u;
-        }
-        ptx::tcgen05_fence_after();
-        fix = *reinterpret_cast<volatile int*>(&sm.special_flag[slot]) != 0;
-        const float inv = it.n_splits > 1 ? 1.f : (l_all == 0.f ? 0.f : 1.0f / l_all);
-        const size_t pr = static_cast<size_t>(it.row0) + static_cast<size_t>(it.split) * rows + tok * group + head;
-#pragma unroll 1
-        for (int c = t * (D / 2); c < (t + 1) * (D / 2); c += 32) {
-          uint32_t o0[32], o1[32];
-          ptx::tmem_ld_32x32b_x32(lanes + 2 * kTile + c, o0);
-          if (n > 1) ptx::tmem_ld_32x32b_x32(lanes + 2 * kTile + D + c, o1);
+        if (both) wait(&sm.o_full[1], t == 0 ? o_other : o_phase, 2);
+        if (t == 0 || both) o_phase ^= 1u;
+        if (t == 1 || both) o_other ^= 1u;
+        col0 = lanes + 2 * kTile;
+        col1 = col0 + D;
+        c0 = t * (D / 2);
+        c1 = c0 + D / 2;
+      }
+      ptx::tcgen05_fence_after();
+      const bool fix = *reinterpret_cast<volatile int*>(&sm.special_flag[slot]) != 0;  // values were taken out of V
+      auto load_sums = [&](int c, float (&v)[32]) {
+        uint32_t o0[32];
+        ptx::tmem_ld_32x32b_x32(col0 + c, o0);
+        if (both) {
+          uint32_t o1[32];
+          ptx::tmem_ld_32x32b_x32(col1 + c, o1);
           ptx::tmem_ld_wait();
-          if (valid) {
-            float v[32];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              v[k] = __uint_as_float(o0[k]) * f0;
-              if (n > 1) v[k] = fmaf(__uint_as_float(o1[k]), f1, v[k]);
-            }
-            if (fix) {
+          for (int k = 0; k < 32; ++k) v[k] = fmaf(__uint_as_float(o1[k]), f1, __uint_as_float(o0[k]) * f0);
+        } else {
+          ptx::tmem_ld_wait();
 #pragma unroll
-              for (int k = 0; k < 32; ++k) v[k] += guard_term(special[c + k], pos - base);
-            }
-            if (it.n_splits > 1) {
-#pragma unroll
-              for (int k = 0; k < 32; k += 4)
-                *reinterpret_cast<float4*>(a.part_o + pr * D + c + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
-            } else {
-#pragma unroll
-              for (int k = 0; k < 32; k += 8)
-                *reinterpret_cast<uint4*>(dst + c + k) =
-                    make_uint4(f2_to_h2(v[k] * inv, v[k + 1] * inv), f2_to_h2(v[k + 2] * inv, v[k + 3] * inv),
-                               f2_to_h2(v[k + 4] * inv, v[k + 5] * inv), f2_to_h2(v[k + 6] * inv, v[k + 7] * inv));
-            }
-          }
-          __syncwarp();  // the next load needs the whole warp
+          for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(o0[k]) * f0;
         }
-        if (it.n_splits > 1 && valid && t == 0)
-          a.part_ml[pr] = make_float2(m_all == -INFINITY ? m_all : m_all * scale, l_all);
+        if (fix) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[k] += guard_term(special[c + k], pos - base);
+        }
+      };
+      const size_t record = static_cast<size_t>(it.part) * slot_rows + my_tok * group + head;
+      const float inv = l == 0.f ? 0.f : 1.0f / l;  // nothing visible: zeros; a NaN sum stays NaN
+#pragma unroll 1
+      for (int c = c0; c < c1; c += 32) {
+        float v[32];
+        load_sums(c, v);
+        if (valid) {
+          if (it.part >= 0)
+            store_part(a.part_o + record * D + c, v);
+          else
+            store_row(dst + c, v, inv, wide);
+        }
+        __syncwarp();  // the next load needs the whole warp
+      }
+      if (it.part >= 0 && valid && (dual || t == 0)) a.part_ml[record] = make_float2(m == -INFINITY ? m : m * scale, l);
+      if (!dual) {
         ptx::tcgen05_fence_before();
         exchange();  // both accumulators have been read: either warpgroup may start the next item
-      }
-      if (it.n_splits > 1) {
-        __threadfence();
-        exchange();
-        if (threadIdx.x == 0) sm.last = atomicAdd(&a.counters[it.counter], 1) == it.n_splits - 1;
-        exchange();
-        if (*reinterpret_cast<volatile int*>(&sm.last)) {
-          __threadfence();
-          for (int r = warp; r < rows; r += kSoftmaxWarps) {
-            const int rt = r / group;
-            merge_row(a, it.row0, rows, r, it.n_splits,
-                      a.out + (static_cast<size_t>(it.q_tok + rt) * a.num_heads + kvh * group + r - rt * group) * D, lane);
-          }
-        }
-        exchange();  // `last` may be overwritten from here on
       }
       if (fix) {  // every warp has read the record: clear it for the slot's next item
         exchange();
@@ -440,137 +707,140 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       release_item();
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-    if (warp == kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 152;");
+    if (warp == kMmaWarp || warp == kMmaWarp + 1) {
       // =============================== MMA issue ===============================
-      constexpr uint32_t idesc_qk = ptx::make_f16_idesc(kTile, kTile);
+      constexpr uint32_t idesc_qk = ptx::make_f16_idesc(kTile, kHalf);
       constexpr uint32_t idesc_pv = ptx::make_f16_idesc(kTile, D) | ptx::kIdescBMnMajor;
-      Ring ring;
-      uint32_t q_phase = 0, p_phase[2] = {0, 0};
-      const uint32_t q_base = ptx::smem_u32(smem + Sh::kQ), kv_base = ptx::smem_u32(smem + Sh::kRing);
-      auto issue_qk = [&](int t, int qt, int stage) {
-        if (ptx::elect_one()) {
+      // One warp per score tile.  The tensor core takes instructions a few deep only, so whatever a warp does
+      // between two groups of products leaves it idle unless the other warp has products for it (one
+      // warp for both tiles took 1.5 times as long), and a single warp executes slowly: the loop is kept
+      // short -- one wait per pair of tiles, one per half -- and uniform over the warp (lengths broadcast, one
+      // elected lane issues), because MMA descriptors come from uniform registers.
+      const int t = warp - kMmaWarp;
+      const uint64_t v_desc = ptx::make_sw128_mnmajor_desc(ptx::smem_u32(smem + Sh::kRing), Sh::kSubBytes);
+      const uint64_t k_desc = ptx::make_sw128_kmajor_desc(ptx::smem_u32(smem + Sh::kRing + Sh::kTileBytes));
+      const uint32_t utmem = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t s_tmem = utmem + t * kTile, o_tmem = utmem + 2 * kTile + t * D;
+      uint32_t q_phase = 0, count = 0, p_phase[2] = {0, 0};
+      // S_t, half b of the keys (one thread).
+      auto qk = [&](uint64_t q_desc, uint32_t stage, int b) {
+        const uint64_t k = k_desc + ((stage * Sh::kPairBytes + b * (kHalf * 128)) >> 4);
 #pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks) {
-            const uint32_t off = (ks >> 2) * Sh::kSubBytes + (ks & 3) * 32;
-            ptx::umma_f16(tmem + t * kTile, ptx::make_sw128_kmajor_desc(q_base + qt * Sh::kTileBytes + off),
-                          ptx::make_sw128_kmajor_desc(kv_base + stage * Sh::kTileBytes + off), idesc_qk, ks > 0);
-          }
-          ptx::umma_commit(&sm.s_full[t]);
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t at = ((ks >> 2) * Sh::kSubBytes + (ks & 3) * 32) >> 4;
+          ptx::umma_f16(s_tmem + b * kHalf, q_desc + at, k + at, idesc_qk, ks > 0);
         }
-        __syncwarp();
+        ptx::umma_commit(&sm.s_full[t][b]);
       };
-      auto issue_pv = [&](int t, int stage, bool accumulate) {
-        if (ptx::elect_one()) {
+      // O_t += P_t V over half b of the keys (one thread).
+      auto pv = [&](uint32_t stage, int b, bool accumulate) {
+        const uint64_t v = v_desc + ((stage * Sh::kPairBytes + b * (kHalf * 128)) >> 4);
 #pragma unroll
-          for (int ks = 0; ks < kTile / 16; ++ks)
-            ptx::umma_f16_ts(tmem + 2 * kTile + t * D, tmem + t * kTile + ks * 8,
-                             ptx::make_sw128_mnmajor_desc(kv_base + stage * Sh::kTileBytes + ks * 2048, Sh::kSubBytes),
-                             idesc_pv, accumulate || ks > 0);
-        }
-        __syncwarp();
+        for (int k = 0; k < kHalf / 16; ++k)
+          ptx::umma_f16_ts(o_tmem, s_tmem + b * kHalf + k * 8, v + (k * 2048 >> 4), idesc_pv, accumulate || k > 0);
       };
-      uint32_t k_phase = 0, v_phase = 0;  // a bit per stage: the barriers of a kind only count that kind's tiles
-      auto wait_k = [&]() {
-        const int ks = ring.stage;
-        wait(&sm.k_full[ks], (k_phase >> ks) & 1u, 1);
-        k_phase ^= 1u << ks;
-        advance<kStages>(ring);
-        return ks;
-      };
-      auto wait_v = [&]() {
-        const int vs = ring.stage;
-        wait(&sm.v_ok[vs], (v_phase >> vs) & 1u, 1);
-        v_phase ^= 1u << vs;
-        advance<kStages>(ring);
-        return vs;
-      };
-      auto commit = [&](uint64_t* bar) {
-        if (ptx::elect_one()) ptx::umma_commit(bar);
-        __syncwarp();
-      };
-      auto wait_p = [&](int t) {
-        wait(&sm.p_full[t], p_phase[t], 1);
-        p_phase[t] ^= 1u;
-        ptx::tcgen05_fence_after();
-      };
-      Item it;
+      Work it;
       while (next_item(it, 1)) {
-        const int n = it.tile1 - it.tile0;
+        const int n = __shfl_sync(0xffffffffu, it.tile1 - it.tile0, 0);
         if (n <= 0) {
           release_item();
           continue;
         }
-        const bool dual = it.n_tok > tile_tokens;
+        const bool dual = __shfl_sync(0xffffffffu, static_cast<int>(it.n_tok > tile_tokens), 0) != 0;
+        const int odd = __shfl_sync(0xffffffffu, static_cast<int>(half_empty(it)), 0);
+        const int ahead = dual ? 1 : 2;  // also the distance between this warp's kv tiles
+        const uint64_t q_desc = ptx::make_sw128_kmajor_desc(ptx::smem_u32(smem + Sh::kQ)) +
+                                (dual ? t * Sh::kTileBytes >> 4 : 0);
         wait(&sm.q_full, q_phase, 1);
         q_phase ^= 1u;
-        const int first = wait_k();
-        ptx::tcgen05_fence_after();
-        issue_qk(0, 0, first);
-        if (dual) issue_qk(1, 1, first);
-        commit(&sm.kv_empty[first]);
-        if (!dual && n > 1) {
-          const int second = wait_k();
-          issue_qk(1, 0, second);
-          commit(&sm.kv_empty[second]);
+        if (!dual && t >= n) {  // no kv tile for this warp, and no use of Q
+          if (lane == 0) ptx::mbar_arrive(&sm.q_empty);
+          __syncwarp();
         }
-        if (n <= (dual ? 1 : 2)) commit(&sm.q_empty);
-        if (dual) {
-          for (int j = 0; j < n; ++j) {
-            const int vs = wait_v();
-            wait_p(0);
-            issue_pv(0, vs, j > 0);
-            int ks = 0;
-            if (j + 1 < n) {
-              ks = wait_k();
-              issue_qk(0, 0, ks);
-            } else {
-              commit(&sm.o_full[0]);
-            }
-            wait_p(1);
-            issue_pv(1, vs, j > 0);
-            commit(&sm.kv_empty[vs]);
-            if (j + 1 < n) {
-              issue_qk(1, 1, ks);
-              commit(&sm.kv_empty[ks]);
-              if (j + 2 == n) commit(&sm.q_empty);
-            } else {
-              commit(&sm.o_full[1]);
-            }
+        for (int p = 0; p < n + ahead; ++p, ++count) {
+          const uint32_t stage = stage_of(count);
+          wait(&sm.pair_ok[stage], phase_of(count), 1);
+          if (!dual && (p & 1) != t) {  // the other warp's
+            if (lane == 0) ptx::mbar_arrive(&sm.pair_empty[stage]);
+            __syncwarp();
+            continue;
           }
-        } else {
-          for (int i = 0; i < n; ++i) {
-            const int t = i & 1;
-            const int vs = wait_v();
-            wait_p(t);
-            issue_pv(t, vs, i > 1);
-            commit(&sm.kv_empty[vs]);
-            if (i + 2 < n) {
-              const int ks = wait_k();
-              issue_qk(t, 0, ks);
-              commit(&sm.kv_empty[ks]);
-              if (i + 3 == n) commit(&sm.q_empty);
-            } else {
-              commit(&sm.o_full[t]);
+          ptx::tcgen05_fence_after();
+          // Two halves of the score tile are under way at any time: while the softmax works on one, the
+          // tensor core adds the one before to the output and computes the one after it.
+          const int k_halves = p >= n ? 0 : (p + 1 == n ? 2 - odd : 2);
+          if (p < ahead) {
+            if (ptx::elect_one()) {
+              if (k_halves > 0) qk(q_desc, stage, 0);
+              if (k_halves > 1) qk(q_desc, stage, 1);
+              ptx::umma_commit(&sm.pair_empty[stage]);
+              if (p < n && p + ahead >= n) ptx::umma_commit(&sm.q_empty);
             }
+            __syncwarp();
+            continue;
+          }
+          const int v_halves = p - ahead + 1 == n ? 2 - odd : 2;
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            if (b >= v_halves) break;
+            wait(&sm.p_full[t][b], p_phase[b], 1);
+            p_phase[b] ^= 1u;
+            ptx::tcgen05_fence_after();
+            if (ptx::elect_one()) {
+              pv(stage, b, p >= 2 * ahead || b > 0);
+              if (b < k_halves) qk(q_desc, stage, b);
+              if (b + 1 == v_halves) {
+                ptx::umma_commit(&sm.pair_empty[stage]);
+                if (p < n && p + ahead >= n) ptx::umma_commit(&sm.q_empty);
+              }
+              if (b >= k_halves) ptx::umma_commit(b + 1 == v_halves && p + ahead >= n + ahead ? &sm.o_full[t] : &sm.pv_done[t]);
+            }
+            __syncwarp();
           }
         }
         release_item();
       }
     } else if (warp == kProducerWarp) {
       // =============================== loads ===============================
-      const int n_items = a.header->n_items;
       const int boxes = kTile / box_tokens;          // per 64-channel sub-tile
       const int my_box = lane / Sh::kHalves, my_half = lane - my_box * Sh::kHalves;
       const bool loads = my_box < boxes;
-      Ring ring;
-      uint32_t q_phase = 0, k_count = 0;
-      int idx = blockIdx.x;
-      while (idx < n_items && !dead) {
-        const Item it = a.items[idx];
-        if (lane == 0) idx = gridDim.x + atomicAdd(&a.header->ticket, 1);
-        idx = __shfl_sync(0xffffffffu, idx, 0);
-        if (it.split >= it.n_splits) continue;
+      uint32_t q_phase = 0, k_count = 0, count = 0;
+      const long long x0 = blockIdx.x * line.share, x1 = x0 + line.share;
+      CutUnit* cut = a.max_rows > 0 ? static_cast<CutUnit*>(a.cuts) + blockIdx.x : nullptr;
+      bool listed = false;
+      Unit u;
+      bool more = sm.found.seq < a.bs;
+      if (more) u = unit_at(a, sm.found, x0);
+      for (; more && u.at < x1 && !dead; more = next_unit(a, u)) {
+        Work it;
+        it.q_tok = u.s.start + u.block * a.block_tokens;
+        it.n_tok = u.n_tok;
+        it.pos0 = u.pos0;
+        it.seq = u.seq;
+        it.head = u.head;
+        it.tile0 = cut_tile(u, x0 - u.at, line.share);
+        it.tile1 = cut_tile(u, x1 - u.at, line.share);
+        // a block without keys (zeros) belongs to the stretch that it starts in
+        if (u.tiles == 0 ? u.at < x0 : it.tile0 >= it.tile1) continue;
+        it.part = it.tile0 == 0 && it.tile1 == u.tiles ? -1 : part_of(u, static_cast<int>(blockIdx.x), line.share);
+        if (it.tile0 == 0 && it.tile1 < u.tiles) {  // first part of a cut unit: list the parts for the merge
+          int n = 0;
+          for (int c = blockIdx.x; c * line.share < u.at + u.length; c += 32) {
+            const int part = (c + lane) * line.share < u.at + u.length ? part_of(u, c + lane, line.share) : -1;
+            const uint32_t has = __ballot_sync(0xffffffffu, part >= 0);
+            if (part >= 0) cut->parts[n + __popc(has & ((1u << lane) - 1u))] = part;
+            n += __popc(has);
+          }
+          if (lane == 0) {
+            cut->n = n;
+            cut->q_tok = it.q_tok;
+            cut->n_tok = it.n_tok;
+            cut->head = it.head;
+          }
+          listed = true;
+        }
         wait(&sm.item_empty[slot], slot_phase ^ 1u, 0);
         if (lane == 0) {
           sm.items[slot] = it;
@@ -592,31 +862,14 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           const int pg = table[first / a.page_size];
           return pg >= 0 && pg < a.num_pages ? pg : a.num_pages;
         };
-        auto load = [&](const CUtensorMap* map, uint64_t* full, int i, int page) {
-          wait(&sm.kv_empty[ring.stage], ring.phase ^ 1u, 0);
-          if (!dead) {
-            if (lane == 0) ptx::mbar_arrive_expect_tx(&full[ring.stage], Sh::kTileBytes);
-            __syncwarp();
-            if (loads)
-              ptx::tma_load_4d(smem + Sh::kRing + ring.stage * Sh::kTileBytes + my_half * Sh::kSubBytes +
-                                   my_box * box_tokens * 128,
-                               map, &full[ring.stage], my_half * 64, it.head,
-                               ((it.tile0 + i) * kTile + my_box * box_tokens) % a.page_size, page);
-          }
-          __syncwarp();
-          advance<kStages>(ring);
+        const int offset0 = my_box * box_tokens;
+        auto load = [&](const CUtensorMap* map, uint32_t stage, int half_of_pair, int i, int page) {
+          ptx::tma_load_4d(smem + Sh::kRing + stage * Sh::kPairBytes + half_of_pair * Sh::kTileBytes +
+                               my_half * Sh::kSubBytes + offset0 * 128,
+                           map, &sm.pair_full[stage], my_half * 64, it.head,
+                           ((it.tile0 + i) * kTile + offset0) % a.page_size, page);
         };
-        auto load_k = [&](int i, int page) {
-          // which keys lie in a page that exists, for the softmax; published by the K tile's barrier
-          const uint32_t per_box = box_tokens / 8;
-          uint32_t bits = 0;
-          if (loads && my_half == 0 && page < a.num_pages)
-            bits = ((1u << per_box) - 1u) << (my_box * per_box);
-          bits = __reduce_or_sync(0xffffffffu, bits);
-          if (lane == 0) sm.valid[(k_count + i) & (kMaskRing - 1)] = bits;
-          load(&map_k, sm.k_full, i, page);
-        };
-        int p0 = page_of(0), p1 = page_of(1), p2;  // pages of the next tiles, read ahead of their use
+        int page = page_of(0), behind[2] = {0, 0};  // pages of tile p, p - 1, p - 2
         // Q: rows (token, head) of this kv head's group
         wait(&sm.q_empty, q_phase ^ 1u, 0);
         q_phase ^= 1u;
@@ -629,31 +882,35 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                                it.head * group, it.q_tok + t * tile_tokens);
         }
         __syncwarp();
-        load_k(0, p0);
-        if (ahead == 2) {
-          p2 = page_of(2);
-          if (n > 1) load_k(1, p1);
-        } else {
-          p2 = 0;
-        }
-        for (int i = 0; i < n; ++i) {
-          load(&map_v, sm.v_full, i, p0);
-          const int next = i + ahead;
-          if (ahead == 2) {
-            const int p3 = page_of(next + 1);
-            if (next < n) load_k(next, p2);
-            p0 = p1;
-            p1 = p2;
-            p2 = p3;
-          } else {
-            const int p3 = page_of(next + 1);
-            if (next < n) load_k(next, p1);
-            p0 = p1;
-            p1 = p3;
+        for (int p = 0; p < n + ahead; ++p, ++count) {
+          const uint32_t stage = stage_of(count);
+          const bool has_k = p < n, has_v = p >= ahead;
+          const int next = page_of(p + 1);  // read ahead of its use
+          if (has_k) {
+            // which keys lie in a page that exists, for the softmax; published by the pair's barrier
+            const uint32_t per_box = box_tokens / 8;
+            uint32_t bits = 0;
+            if (loads && my_half == 0 && page < a.num_pages) bits = ((1u << per_box) - 1u) << (my_box * per_box);
+            bits = __reduce_or_sync(0xffffffffu, bits);
+            if (lane == 0) sm.valid[(k_count + p) & (kMaskRing - 1)] = bits;
           }
+          wait(&sm.pair_empty[stage], phase_of(count) ^ 1u, 0);
+          if (!dead) {
+            if (lane == 0) ptx::mbar_arrive_expect_tx(&sm.pair_full[stage], (has_k + has_v) * Sh::kTileBytes);
+            __syncwarp();
+            if (loads) {
+              if (has_v) load(&map_v, stage, 0, p - ahead, behind[ahead - 1]);
+              if (has_k) load(&map_k, stage, 1, p, page);
+            }
+          }
+          __syncwarp();
+          behind[1] = behind[0];
+          behind[0] = page;
+          page = next;
         }
         k_count += n;
       }
+      if (cut != nullptr && !listed && lane == 0) cut->n = 0;
       if (!dead) {  // the end mark
         wait(&sm.item_empty[slot], slot_phase ^ 1u, 0);
         if (lane == 0) {
@@ -663,47 +920,51 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       }
     } else {
       // =============================== V guard ===============================
-      const int part = warp - kGuardWarp;  // this warp's half of the rows
-      uint32_t v_phase = 0;
-      Ring ring;
-      Item it;
+      uint32_t count = 0;
+      Work it;
       while (next_item(it, 3)) {
         const int n = it.tile1 - it.tile0;
-        const bool dual = it.n_tok > tile_tokens;
+        const int ahead = it.n_tok > tile_tokens ? 1 : 2;
         const int kv_len = it.pos0 + it.n_tok;
         uint32_t* special = sm.special[slot];
-        if (n > 0) advance<kStages>(ring);  // over the K tiles
-        if (!dual && n > 1) advance<kStages>(ring);
-        for (int i = 0; i < n; ++i) {
-          wait(&sm.v_full[ring.stage], (v_phase >> ring.stage) & 1u, 3);
-          v_phase ^= 1u << ring.stage;
-          const int t0 = (it.tile0 + i) * kTile;
-          uint8_t* tile = smem + Sh::kRing + ring.stage * Sh::kTileBytes;
+        for (int p = 0; n > 0 && p < n + ahead; ++p, ++count) {
+          const uint32_t stage = stage_of(count);
+          wait(&sm.pair_full[stage], phase_of(count), 3);
+          // (a pair without a V tile: nothing lies at or behind hid)
+          const int t0 = p < ahead ? -0x40000000 : (it.tile0 + p - ahead) * kTile;
+          uint8_t* tile = smem + Sh::kRing + stage * Sh::kPairBytes;
           // rows behind the context: zeros (whole rows, so the swizzle does not matter)
           const int end = min(max(kv_len - t0, 0), kTile);
           // rows that some row of the block does not see: no infinities, no NaN
           const int hid = min(max(it.pos0 + 1 - t0, 0), end);
           if (hid < kTile) {
-            const int lo = max(hid, part * (kTile / 2)), hi = (part + 1) * (kTile / 2);
-            for (int k = lo * (D / 8) + lane; k < hi * (D / 8); k += 32) {
-              const int r = k / (D / 8), c = k - r * (D / 8);
-              uint4* p = reinterpret_cast<uint4*>(tile + (c >> 3) * Sh::kSubBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-              if (r >= end) {
-                *p = make_uint4(0, 0, 0, 0);
-              } else {
-                uint4 v = *p;
-                if (any_nonfinite(v)) {
-                  guard_take(v, static_cast<uint32_t>(t0 + r - (it.pos0 + 1)), special + c * 8, &sm.special_flag[slot]);
-                  *p = v;
+            constexpr int kChunks = D / 8, kAhead = 4;  // loads under way per lane
+            for (int k0 = hid * kChunks + lane; k0 < kTile * kChunks; k0 += 32 * kAhead) {
+              uint4 v[kAhead];
+#pragma unroll
+              for (int u = 0; u < kAhead; ++u) {
+                const int k = min(k0 + 32 * u, kTile * kChunks - 1);
+                const int r = k / kChunks, c = k - r * kChunks;
+                v[u] = *reinterpret_cast<const uint4*>(tile + (c >> 3) * Sh::kSubBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+              }
+#pragma unroll
+              for (int u = 0; u < kAhead; ++u) {
+                const int k = k0 + 32 * u;
+                if (k >= kTile * kChunks) break;
+                const int r = k / kChunks, c = k - r * kChunks;
+                uint4* p = reinterpret_cast<uint4*>(tile + (c >> 3) * Sh::kSubBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+                if (r >= end) {
+                  *p = make_uint4(0, 0, 0, 0);
+                } else if (any_nonfinite(v[u])) {
+                  guard_take(v[u], static_cast<uint32_t>(t0 + r - (it.pos0 + 1)), special + c * 8, &sm.special_flag[slot]);
+                  *p = v[u];
                 }
               }
             }
             ptx::fence_proxy_async();
           }
           __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(&sm.v_ok[ring.stage]);
-          advance<kStages>(ring);
-          if (i + (dual ? 1 : 2) < n) advance<kStages>(ring);
+          if (lane == 0) ptx::mbar_arrive(&sm.pair_ok[stage]);
         }
         release_item();
       }
@@ -726,6 +987,81 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   }
 }
 
+// ---- merge of cut units ---------------------------------------------------------------------
+constexpr int kMergeThreads = 256;
+constexpr int kMergeRows = 4;  // rows a warp takes at once: their loads overlap
+
+// CTA (c, y): a share of the rows of the unit whose first part CTA c of the attention had.  Every row is
+// sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over its parts, in their order.  A chain of three L2 round
+// trips (the list, the maxima, the sums); bound by reading the records (D + 2 floats per row and part).
+template <int D>
+__global__ void __launch_bounds__(kMergeThreads) chunk_attention_merge_kernel(const Args a) {
+  constexpr int kPer = D / 32;  // channels per lane
+  pdl_trigger();
+  pdl_wait();
+  const CutUnit& cut = static_cast<const CutUnit*>(a.cuts)[blockIdx.x];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n = cut.n, rows = cut.n_tok * a.group;
+  const int r0 = (blockIdx.y * (kMergeThreads / 32) + warp) * kMergeRows;
+  if (n == 0 || r0 >= rows) return;
+  float m[kMergeRows], l[kMergeRows], acc[kMergeRows][kPer];
+#pragma unroll
+  for (int j = 0; j < kMergeRows; ++j) {
+    m[j] = -INFINITY;
+    l[j] = 0.f;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) acc[j][k] = 0.f;
+  }
+  for (int i = lane; i < n; i += 32) {
+    const float2* ml = a.part_ml + static_cast<size_t>(cut.parts[i]) * a.slot_rows;
+#pragma unroll
+    for (int j = 0; j < kMergeRows; ++j) m[j] = fmaxf(m[j], ml[min(r0 + j, rows - 1)].x);
+  }
+#pragma unroll
+  for (int j = 0; j < kMergeRows; ++j) {
+    m[j] = warp_max(m[j]);
+    if (m[j] == -INFINITY) m[j] = 0.f;
+  }
+#pragma unroll 2
+  for (int i = 0; i < n; ++i) {
+    const size_t pr = static_cast<size_t>(cut.parts[i]) * a.slot_rows;
+#pragma unroll
+    for (int j = 0; j < kMergeRows; ++j) {
+      const int r = min(r0 + j, rows - 1);
+      const float2 ml = a.part_ml[pr + r];
+      const float w = exp2f(ml.x - m[j]);
+      l[j] += ml.y * w;
+      float v[kPer];
+      const float* src = a.part_o + (pr + r) * D + lane * kPer;
+      if constexpr (kPer == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(src);
+        v[0] = x.x;
+        v[1] = x.y;
+        v[2] = x.z;
+        v[3] = x.w;
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(src);
+        v[0] = x.x;
+        v[1] = x.y;
+      }
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) acc[j][k] = fmaf(w, w != 0.f ? v[k] : 0.f, acc[j][k]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kMergeRows; ++j) {
+    const int r = r0 + j;
+    if (r >= rows) break;
+    const float inv = l[j] == 0.f ? 0.f : 1.0f / l[j];  // nothing visible: zeros; a NaN sum stays NaN
+    const int tok = r / a.group;
+    __half* dst = a.out + (static_cast<size_t>(cut.q_tok + tok) * a.num_heads + cut.head * a.group + r - tok * a.group) * D + lane * kPer;
+    if constexpr (kPer == 4)
+      *reinterpret_cast<uint2*>(dst) = make_uint2(f2_to_h2(acc[j][0] * inv, acc[j][1] * inv), f2_to_h2(acc[j][2] * inv, acc[j][3] * inv));
+    else
+      *reinterpret_cast<uint32_t*>(dst) = f2_to_h2(acc[j][0] * inv, acc[j][1] * inv);
+  }
+}
+
 int box_tokens_of(int page_size) {
   for (int b = 128; b >= 8; b >>= 1)
     if (page_size % b == 0) return b;
@@ -738,7 +1074,7 @@ int launch_tc_d(const Args& a, cudaStream_t st) {
   const uint64_t e = 2;
   const int box = box_tokens_of(a.page_size);
   {
-    const uint64_t dims[3] = {D, static_cast<uint64_t>(a.num_heads), static_cast<uint64_t>(a.num_tokens)};
+    const uint64_t dims[3] = {static_cast<uint64_t>(D), static_cast<uint64_t>(a.num_heads), static_cast<uint64_t>(a.num_tokens)};
     const uint64_t strides[2] = {D * e, static_cast<uint64_t>(a.num_heads) * D * e};
     const uint32_t b[3] = {64, static_cast<uint32_t>(a.group), static_cast<uint32_t>(a.block_tokens / 2)};
     const int rc = encode_f16_map(&mq, a.q, 3, dims, strides, b, "chunked_paged_attention(q)");
@@ -746,7 +1082,7 @@ int launch_tc_d(const Args& a, cudaStream_t st) {
   }
   {
     const uint64_t hkv = a.num_kv_heads, page = a.page_size;
-    const uint64_t dims[4] = {D, hkv, page, static_cast<uint64_t>(a.num_pages)};
+    const uint64_t dims[4] = {static_cast<uint64_t>(D), hkv, page, static_cast<uint64_t>(a.num_pages)};
     const uint64_t strides[3] = {D * e, hkv * D * e, page * hkv * D * e};
     const uint32_t b[4] = {64, 1, static_cast<uint32_t>(box), 1};
     int rc = encode_f16_map(&mk, a.k_cache, 4, dims, strides, b, "chunked_paged_attention(key_cache)");
@@ -762,12 +1098,18 @@ int launch_tc_d(const Args& a, cudaStream_t st) {
     B200OPS_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes<D>())));
     if (dev >= 0 && dev < 64) attr_set[dev].store(true, std::memory_order_release);
   }
-  const int grid = a.max_items < sm_count() ? a.max_items : sm_count();
-  B200OPS_CUDA(launch_kernel(kern, dim3(grid), dim3(kThreads), smem_bytes<D>(), st, mq, mk, mv, a, box));
+  B200OPS_CUDA(launch_kernel(kern, dim3(a.shares), dim3(kThreads), smem_bytes<D>(), st, mq, mk, mv, a, box));
+  if (a.max_rows > 0) {  // some context may be long enough to be cut
+    constexpr int kRowsPerCta = kMergeThreads / 32 * kMergeRows;
+    B200OPS_CUDA(launch_kernel(chunk_attention_merge_kernel<D>, dim3(a.shares, (a.slot_rows + kRowsPerCta - 1) / kRowsPerCta),
+                               dim3(kMergeThreads), 0, st, a));
+  }
   return B200OPS_OK;
 }
 
 }  // namespace
+
+size_t cut_list_bytes(int shares) { return static_cast<size_t>(shares) * sizeof(CutUnit); }
 
 bool tc_supported(int64_t head_dim, int64_t group, int64_t page_size, int layout) {
   return (head_dim == 64 || head_dim == 128) && group <= 128 && page_size % 8 == 0 && layout == B200OPS_KV_LAYOUT_NHD;
