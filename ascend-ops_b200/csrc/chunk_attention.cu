@@ -415,11 +415,11 @@ void plan_shape(Args* a, bool tc) {
     a->group = group;
     a->head_tiles = 1;
     a->block_tokens = 2 * (128 / group);
-    a->kv_tile = 128;
+    a->kv_tile = 64;
     a->shares = sm_count() < kMaxShares ? sm_count() : kMaxShares;
     a->slot_rows = (a->block_tokens < a->num_tokens ? a->block_tokens : a->num_tokens) * group;
     // two records per stretch, unless no context is long enough to be cut
-    const bool cut = a->shares > 1 && static_cast<int64_t>(a->max_pages_per_seq) * a->page_size > 3 * a->kv_tile;
+    const bool cut = a->shares > 1 && static_cast<int64_t>(a->max_pages_per_seq) * a->page_size > 5 * a->kv_tile;
     a->max_rows = cut ? 2 * a->shares * a->slot_rows : 0;
     return;
   } else {

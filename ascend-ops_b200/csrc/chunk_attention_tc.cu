@@ -33,8 +33,8 @@ namespace ca {
 namespace {
 
 constexpr int kThreads = 384;
-constexpr int kTile = 128;  // keys per kv tile, rows per score tile
-constexpr int kHalf = 64;   // keys per score buffer
+constexpr int kRows = 128;  // rows of a score tile
+constexpr int kKeys = 64;   // keys of a kv tile
 constexpr int kMaskRing = 16;
 constexpr int kMmaWarp = 8, kProducerWarp = 10, kGuardWarp = 11;  // MMA: 8 and 9, one per score tile
 constexpr uint32_t kSoftmaxWarps = 8;
@@ -92,8 +92,8 @@ __device__ __forceinline__ void set_block(const Args& a, Unit& u) {
 __device__ __forceinline__ int cut_tile(const Unit& u, long long x, long long share) {
   if (x <= 0) return 0;
   if (x >= u.length) return u.tiles;
-  // Short shares (small batches): parts of four tiles, or the merge costs more than the parts save.
-  const int grain = share >= 4096 ? 1 : 4, least = share >= 4096 ? 2 : 4;
+  // Short shares (small batches): parts of eight tiles, or the merge costs more than the parts save.
+  const int grain = share >= 4096 ? 1 : 8, least = share >= 4096 ? 3 : 8;
   // fp32 with each operation rounded by itself: cheaper than a 64-bit division, the same in both
   // kernels, and it never decreases in x
   int k = min(static_cast<int>(__fdiv_rn(__fmul_rn(static_cast<float>(x), static_cast<float>(u.tiles)),
@@ -183,11 +183,6 @@ struct Work {
   int part;  // record to write (see part_of); -1: the unit is whole, write the result
 };
 
-// Whether the second half of the last kv tile lies behind every key that the block sees.
-__device__ __forceinline__ bool half_empty(const Work& w) {
-  return w.pos0 + w.n_tok - (w.tile1 - 1) * kTile <= kHalf;
-}
-
 // A cut unit, as the merge needs it; left by the CTA that has its first part (n = 0: none).
 struct CutUnit {
   int n, q_tok, n_tok, head;
@@ -204,20 +199,22 @@ __device__ __forceinline__ int part_of(const Unit& u, int c, long long share) {
 template <int D>
 struct Shape {
   static constexpr int kHalves = D / 64;                    // 64-channel sub-tiles
-  static constexpr int kSubBytes = kTile * 128;             // [128 rows][64 halfs]
-  static constexpr int kTileBytes = kHalves * kSubBytes;    // one Q, K or V tile
+  static constexpr int kQSub = kRows * 128;                 // [128 rows][64 halfs]
+  static constexpr int kQBytes = kHalves * kQSub;
+  static constexpr int kSub = kKeys * 128;                  // [64 keys][64 halfs]
+  static constexpr int kTileBytes = kHalves * kSub;         // one K or V tile
   static constexpr int kPairBytes = 2 * kTileBytes;         // a V tile, then the K tile that goes with it
-  static constexpr int kStages = D == 128 ? 2 : 4;          // pairs in the ring, a power of two
+  static constexpr int kStages = D == 128 ? 5 : 10;         // pairs in the ring
   static constexpr int kQ = 0;
-  static constexpr int kRing = 2 * kTileBytes;
+  static constexpr int kRing = 2 * kQBytes;
   static constexpr int kMeta = kRing + kStages * kPairBytes;
 };
 
 struct Meta {
   uint64_t item_full[2], item_empty[2];
   uint64_t q_full, q_empty;
-  uint64_t pair_full[4], pair_ok[4], pair_empty[4];  // landed; looked over by the guard; used up
-  uint64_t s_full[2][2], p_full[2][2];  // [score tile][half of the keys]
+  uint64_t pair_full[10], pair_ok[10], pair_empty[10];  // landed; looked over by the guard; used up
+  uint64_t s_full[2][2], p_full[2][2];  // [score tile][buffer]
   uint64_t pv_done[2], o_full[2];        // after an item's last but one and last second product
   uint64_t exchange;  // the softmax warps' barrier (bounded, unlike bar.sync)
   uint32_t tmem_base;
@@ -227,7 +224,7 @@ struct Meta {
   Found found;
   long long sums[32];
   uint32_t valid[kMaskRing];     // per kv tile: bit i = keys 8i .. 8i+7 lie in a page that exists
-  float swap[2][kTile];          // per tile and row: maxima, then sums, of a block of one score tile
+  float swap[2][kRows];          // per tile and row: maxima, then sums, of a block of one score tile
   uint32_t special[2][128];      // per item slot and channel: packed positions, see guard
 };
 
@@ -431,10 +428,15 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   };
 
   // Pair p of an item: K tile p and V tile p - ahead, the two that one step of the MMA loop reads (the
-  // first `ahead` pairs have no V, the last ones no K).  Pair number c of the CTA lies in stage
-  // c mod kStages.
-  auto stage_of = [](uint32_t c) { return c & (kStages - 1); };
-  auto phase_of = [](uint32_t c) { return (c / kStages) & 1u; };
+  // first `ahead` pairs have no V, the last ones no K).  The pairs of all items go round one ring of stages.
+  int stage = 0;
+  uint32_t phase = 0;
+  auto next_stage = [&]() {
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  };
 
   // Items arrive through a two-slot ring.
   int slot = 0;
@@ -457,8 +459,8 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     const int t = warp >> 2;                    // score tile
     const int row = (warp & 3) * 32 + lane;     // row of the tile = TMEM lane
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t s_col = lanes + t * kTile;
-    const uint32_t o_col = lanes + 2 * kTile + t * D;
+    const uint32_t s_col = lanes + t * 2 * kKeys;
+    const uint32_t o_col = lanes + 4 * kKeys + t * D;
     uint32_t s_phase = 0, o_phase = 0, x_phase = 0, o_other = 0;  // s_phase: a bit per half
     uint32_t pv_phase = 0;
     uint32_t k_count = 0;  // kv tiles before this item
@@ -487,29 +489,27 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         release_item();
         continue;
       }
-      // Halves of kv tiles that this warpgroup sees; the last tile's second half may hold no key at all.
-      const int my_n = dual ? n : (n + 1 - t) / 2;
-      const int halves = 2 * my_n - (half_empty(it) && (dual || t == ((n - 1) & 1)) ? 1 : 0);
+      const int steps = dual ? n : (n + 1 - t) / 2;  // kv tiles of this warpgroup
       float m = -INFINITY, l = 0.f;  // reference maximum (raw scores) and sum
       float limit = -INFINITY;       // scores up to here keep the reference
-      const int row_pos = pos - it.tile0 * kTile;               // this row's position behind the first key
+      const int row_pos = pos - it.tile0 * kKeys;                 // this row's position behind the first key
       const int warp_pos = __shfl_sync(0xffffffffu, row_pos, 0);  // the least of the warp's
-      int off = dual ? 0 : t * kTile;                           // first key of the half
+      int off = dual ? 0 : t * kKeys;                             // first key of the tile
       auto await_scores = [&](int b) {
         wait(&sm.s_full[t][b], (s_phase >> b) & 1u, 2);
         s_phase ^= 1u << b;
         ptx::tcgen05_fence_after();
       };
       auto load_scores = [&](int b, uint32_t (&s)[2][32]) {
-        ptx::tmem_ld_32x32b_x32(s_col + b * kHalf, s[0]);
-        ptx::tmem_ld_32x32b_x32(s_col + b * kHalf + 32, s[1]);
+        ptx::tmem_ld_32x32b_x32(s_col + b * kKeys, s[0]);
+        ptx::tmem_ld_32x32b_x32(s_col + b * kKeys + 32, s[1]);
       };
-      // Half i of the keys, whose scores are in s; leaves those of the next half there.
+      // Tile i, whose scores are in s; leaves those of the next tile there.
       auto step = [&](int i, uint32_t (&s)[2][32]) {
         const int b = i & 1;
-        const uint32_t ok = (sm.valid[(k_count + (off >> 7)) & (kMaskRing - 1)] >> (8 * b)) & 0xffu;
-        if (ok != 0xffu || warp_pos - off < kHalf - 1) {
-          const int last_col = row_pos - off;  // last visible key of the half
+        const uint32_t ok = sm.valid[(k_count + off / kKeys) & (kMaskRing - 1)];
+        if (ok != 0xffu || warp_pos - off < kKeys - 1) {
+          const int last_col = row_pos - off;  // last visible key of the tile
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
             const int vis = min(max(last_col + 1 - g * 32, 0), 32);
@@ -521,7 +521,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
               if (!((bits >> c) & 1u)) s[g][c] = __float_as_uint(-INFINITY);
           }
         }
-        off += b == 0 || dual ? kHalf : 2 * kTile - kHalf;
+        off += dual ? kKeys : 2 * kKeys;
         uint32_t p[32];
         const uint64_t scale2 = pair(scale, scale);
         uint64_t sum2[2];
@@ -546,7 +546,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           }
         };
         // The reference maximum is nearly always still good: the first exponentials are taken with it while
-        // the half's own maximum is being found, and again in the rare case that it was not.
+        // the tile's own maximum is being found, and again in the rare case that it was not.
         exponentials(0, 16);
         float mx[2];
 #pragma unroll
@@ -567,9 +567,9 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             l *= f;
           }
           if (i > 0) {
-            // The accumulator follows, once the product before this one is in it: the next half's scores are
-            // computed behind that product; behind the last half, its own barrier tells.
-            if (i + 1 < halves)
+            // The accumulator follows, once the product before this one is in it: the next tile's scores are
+            // computed behind that product; behind the last tile, its own barrier tells.
+            if (i + 1 < steps)
               wait(&sm.s_full[t][b ^ 1], (s_phase >> (b ^ 1)) & 1u, 2);
             else
               wait(&sm.pv_done[t], pv_phase, 2);
@@ -591,12 +591,12 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         split(add2(sum2[0], sum2[1]), x, y);
         l += x + y;
         // The next scores are on their way while the probabilities are stored (they were issued behind the
-        // product before this half's, so waiting for them first holds nothing up).
-        if (i + 1 < halves) {
+        // product before this tile's, so waiting for them first holds nothing up).
+        if (i + 1 < steps) {
           await_scores(b ^ 1);
           load_scores(b ^ 1, s);
         }
-        ptx::tmem_st_32x32b_x32(s_col + b * kHalf, p);
+        ptx::tmem_st_32x32b_x32(s_col + b * kKeys, p);
         ptx::tmem_st_wait();
         ptx::tcgen05_fence_before();
         __syncwarp();
@@ -604,19 +604,19 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         ptx::tmem_ld_wait();
       };
       if (!__any_sync(0xffffffffu, valid)) {  // no row of this warp is anybody's: its P may be anything
-        for (int i = 0; i < halves; ++i) {
+        for (int i = 0; i < steps; ++i) {
           await_scores(i & 1);
           if (lane == 0) ptx::mbar_arrive(&sm.p_full[t][i & 1]);
         }
-      } else if (halves > 0) {
+      } else if (steps > 0) {
         uint32_t s[2][32];
         await_scores(0);
         load_scores(0, s);
         ptx::tmem_ld_wait();
 #pragma unroll 1
-        for (int i = 0; i < halves; ++i) step(i, s);
+        for (int i = 0; i < steps; ++i) step(i, s);
       }
-      if (halves > 1) pv_phase ^= 1u;
+      if (steps > 1) pv_phase ^= 1u;
       k_count += n;
 
       // ------------------------------ the item's result ------------------------------
@@ -654,7 +654,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         if (both) wait(&sm.o_full[1], t == 0 ? o_other : o_phase, 2);
         if (t == 0 || both) o_phase ^= 1u;
         if (t == 1 || both) o_other ^= 1u;
-        col0 = lanes + 2 * kTile;
+        col0 = lanes + 4 * kKeys;
         col1 = col0 + D;
         c0 = t * (D / 2);
         c1 = c0 + D / 2;
@@ -710,36 +710,19 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     asm volatile("setmaxnreg.dec.sync.aligned.u32 152;");
     if (warp == kMmaWarp || warp == kMmaWarp + 1) {
       // =============================== MMA issue ===============================
-      constexpr uint32_t idesc_qk = ptx::make_f16_idesc(kTile, kHalf);
-      constexpr uint32_t idesc_pv = ptx::make_f16_idesc(kTile, D) | ptx::kIdescBMnMajor;
+      constexpr uint32_t idesc_qk = ptx::make_f16_idesc(kRows, kKeys);
+      constexpr uint32_t idesc_pv = ptx::make_f16_idesc(kRows, D) | ptx::kIdescBMnMajor;
       // One warp per score tile.  The tensor core takes instructions a few deep only, so whatever a warp does
       // between two groups of products leaves it idle unless the other warp has products for it (one
       // warp for both tiles took 1.5 times as long), and a single warp executes slowly: the loop is kept
       // short -- one wait per pair of tiles, one per half -- and uniform over the warp (lengths broadcast, one
       // elected lane issues), because MMA descriptors come from uniform registers.
       const int t = warp - kMmaWarp;
-      const uint64_t v_desc = ptx::make_sw128_mnmajor_desc(ptx::smem_u32(smem + Sh::kRing), Sh::kSubBytes);
+      const uint64_t v_desc = ptx::make_sw128_mnmajor_desc(ptx::smem_u32(smem + Sh::kRing), Sh::kSub);
       const uint64_t k_desc = ptx::make_sw128_kmajor_desc(ptx::smem_u32(smem + Sh::kRing + Sh::kTileBytes));
       const uint32_t utmem = __shfl_sync(0xffffffffu, tmem, 0);
-      const uint32_t s_tmem = utmem + t * kTile, o_tmem = utmem + 2 * kTile + t * D;
-      uint32_t q_phase = 0, count = 0, p_phase[2] = {0, 0};
-      // S_t, half b of the keys (one thread).
-      auto qk = [&](uint64_t q_desc, uint32_t stage, int b) {
-        const uint64_t k = k_desc + ((stage * Sh::kPairBytes + b * (kHalf * 128)) >> 4);
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t at = ((ks >> 2) * Sh::kSubBytes + (ks & 3) * 32) >> 4;
-          ptx::umma_f16(s_tmem + b * kHalf, q_desc + at, k + at, idesc_qk, ks > 0);
-        }
-        ptx::umma_commit(&sm.s_full[t][b]);
-      };
-      // O_t += P_t V over half b of the keys (one thread).
-      auto pv = [&](uint32_t stage, int b, bool accumulate) {
-        const uint64_t v = v_desc + ((stage * Sh::kPairBytes + b * (kHalf * 128)) >> 4);
-#pragma unroll
-        for (int k = 0; k < kHalf / 16; ++k)
-          ptx::umma_f16_ts(o_tmem, s_tmem + b * kHalf + k * 8, v + (k * 2048 >> 4), idesc_pv, accumulate || k > 0);
-      };
+      const uint32_t s_tmem = utmem + t * 2 * kKeys, o_tmem = utmem + 4 * kKeys + t * D;
+      uint32_t q_phase = 0, p_phase = 0;  // p_phase: a bit per buffer
       Work it;
       while (next_item(it, 1)) {
         const int n = __shfl_sync(0xffffffffu, it.tile1 - it.tile0, 0);
@@ -748,68 +731,68 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           continue;
         }
         const bool dual = __shfl_sync(0xffffffffu, static_cast<int>(it.n_tok > tile_tokens), 0) != 0;
-        const int odd = __shfl_sync(0xffffffffu, static_cast<int>(half_empty(it)), 0);
-        const int ahead = dual ? 1 : 2;  // also the distance between this warp's kv tiles
+        const int every = dual ? 1 : 2;  // of the kv tiles, this warp has each, or those of its parity
+        const int ahead = 2 * every;     // two score buffers
         const uint64_t q_desc = ptx::make_sw128_kmajor_desc(ptx::smem_u32(smem + Sh::kQ)) +
-                                (dual ? t * Sh::kTileBytes >> 4 : 0);
+                                (dual ? t * Sh::kQBytes >> 4 : 0);
         wait(&sm.q_full, q_phase, 1);
         q_phase ^= 1u;
         if (!dual && t >= n) {  // no kv tile for this warp, and no use of Q
           if (lane == 0) ptx::mbar_arrive(&sm.q_empty);
           __syncwarp();
         }
-        for (int p = 0; p < n + ahead; ++p, ++count) {
-          const uint32_t stage = stage_of(count);
-          wait(&sm.pair_ok[stage], phase_of(count), 1);
+        uint32_t b = 0;  // score buffer
+        for (int p = 0; p < n + ahead; ++p, next_stage()) {
+          wait(&sm.pair_ok[stage], phase, 1);
           if (!dual && (p & 1) != t) {  // the other warp's
             if (lane == 0) ptx::mbar_arrive(&sm.pair_empty[stage]);
             __syncwarp();
             continue;
           }
+          // Two tiles' scores are under way at any time: while the softmax works on one, the tensor core adds
+          // the one before to the output and computes the one after it.
+          if (p >= ahead) {
+            wait(&sm.p_full[t][b], (p_phase >> b) & 1u, 1);
+            p_phase ^= 1u << b;
+          }
           ptx::tcgen05_fence_after();
-          // Two halves of the score tile are under way at any time: while the softmax works on one, the
-          // tensor core adds the one before to the output and computes the one after it.
-          const int k_halves = p >= n ? 0 : (p + 1 == n ? 2 - odd : 2);
-          if (p < ahead) {
-            if (ptx::elect_one()) {
-              if (k_halves > 0) qk(q_desc, stage, 0);
-              if (k_halves > 1) qk(q_desc, stage, 1);
-              ptx::umma_commit(&sm.pair_empty[stage]);
-              if (p < n && p + ahead >= n) ptx::umma_commit(&sm.q_empty);
-            }
-            __syncwarp();
-            continue;
-          }
-          const int v_halves = p - ahead + 1 == n ? 2 - odd : 2;
+          if (ptx::elect_one()) {
+            if (p >= ahead) {  // O_t += P_t V
+              const uint64_t v = v_desc + (stage * Sh::kPairBytes >> 4);
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            if (b >= v_halves) break;
-            wait(&sm.p_full[t][b], p_phase[b], 1);
-            p_phase[b] ^= 1u;
-            ptx::tcgen05_fence_after();
-            if (ptx::elect_one()) {
-              pv(stage, b, p >= 2 * ahead || b > 0);
-              if (b < k_halves) qk(q_desc, stage, b);
-              if (b + 1 == v_halves) {
-                ptx::umma_commit(&sm.pair_empty[stage]);
-                if (p < n && p + ahead >= n) ptx::umma_commit(&sm.q_empty);
-              }
-              if (b >= k_halves) ptx::umma_commit(b + 1 == v_halves && p + ahead >= n + ahead ? &sm.o_full[t] : &sm.pv_done[t]);
+              for (int k = 0; k < kKeys / 16; ++k)
+                ptx::umma_f16_ts(o_tmem, s_tmem + b * kKeys + k * 8, v + (k * 2048 >> 4), idesc_pv,
+                                 p >= ahead + every || k > 0);
             }
-            __syncwarp();
+            if (p < n) {  // S_t = Q_t K^T
+              const uint64_t k = k_desc + (stage * Sh::kPairBytes >> 4);
+#pragma unroll
+              for (int ks = 0; ks < D / 16; ++ks)
+                ptx::umma_f16(s_tmem + b * kKeys, q_desc + (((ks >> 2) * Sh::kQSub + (ks & 3) * 32) >> 4),
+                              k + (((ks >> 2) * Sh::kSub + (ks & 3) * 32) >> 4), idesc_qk, ks > 0);
+              ptx::umma_commit(&sm.s_full[t][b]);
+            }
+            ptx::umma_commit(&sm.pair_empty[stage]);
+            if (p < n && p + every >= n) ptx::umma_commit(&sm.q_empty);
+            if (p >= n && p >= ahead) ptx::umma_commit(p + every >= n + ahead ? &sm.o_full[t] : &sm.pv_done[t]);
           }
+          __syncwarp();
+          b ^= 1u;
         }
         release_item();
       }
     } else if (warp == kProducerWarp) {
       // =============================== loads ===============================
-      const int boxes = kTile / box_tokens;          // per 64-channel sub-tile
+      const int boxes = kKeys / box_tokens;  // per 64-channel sub-tile
       const int my_box = lane / Sh::kHalves, my_half = lane - my_box * Sh::kHalves;
       const bool loads = my_box < boxes;
-      uint32_t q_phase = 0, k_count = 0, count = 0;
+      const int key0 = my_box * box_tokens;  // of this lane's box in the tile
+      const int skip_pages = kKeys / a.page_size, skip_keys = kKeys % a.page_size;
+      uint32_t q_phase = 0, k_count = 0;
       const long long x0 = blockIdx.x * line.share, x1 = x0 + line.share;
       CutUnit* cut = a.max_rows > 0 ? static_cast<CutUnit*>(a.cuts) + blockIdx.x : nullptr;
       bool listed = false;
+      const uint64_t policy = ptx::l2_evict_first();
       Unit u;
       bool more = sm.found.seq < a.bs;
       if (more) u = unit_at(a, sm.found, x0);
@@ -852,24 +835,40 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         const int n = it.tile1 - it.tile0;
         if (n <= 0) continue;
         const bool dual = it.n_tok > tile_tokens;
-        const int ahead = dual ? 1 : 2;
+        const int ahead = dual ? 2 : 4;
+        // The only block of its sequence reads the keys once; they make room in L2 for those that other
+        // blocks read again.
+        const bool once = u.s.blocks == 1;
         const int kv_len = it.pos0 + it.n_tok;
         const int32_t* table = a.block_tables + static_cast<size_t>(it.seq) * a.max_pages_per_seq;
-        // Page of this lane's box of kv tile i (num_pages: nothing there, TMA fills zeros).
-        auto page_of = [&](int i) {
-          const int first = (it.tile0 + i) * kTile + my_box * box_tokens;
-          if (!loads || i >= n || first >= kv_len) return a.num_pages;
-          const int pg = table[first / a.page_size];
-          return pg >= 0 && pg < a.num_pages ? pg : a.num_pages;
+        // This lane's box of one tile after the other: its page (num_pages: nothing there, TMA fills zeros) and
+        // its place in it.
+        struct Walk {
+          int key, index, offset, page;
         };
-        const int offset0 = my_box * box_tokens;
-        auto load = [&](const CUtensorMap* map, uint32_t stage, int half_of_pair, int i, int page) {
-          ptx::tma_load_4d(smem + Sh::kRing + stage * Sh::kPairBytes + half_of_pair * Sh::kTileBytes +
-                               my_half * Sh::kSubBytes + offset0 * 128,
-                           map, &sm.pair_full[stage], my_half * 64, it.head,
-                           ((it.tile0 + i) * kTile + offset0) % a.page_size, page);
+        auto look = [&](Walk& w) {
+          w.page = a.num_pages;
+          if (loads && w.key < kv_len && w.key < it.tile1 * kKeys) {
+            const int pg = table[w.index];
+            if (pg >= 0 && pg < a.num_pages) w.page = pg;
+          }
         };
-        int page = page_of(0), behind[2] = {0, 0};  // pages of tile p, p - 1, p - 2
+        auto forward = [&](Walk& w) {
+          w.key += kKeys;
+          w.index += skip_pages;
+          w.offset += skip_keys;
+          if (w.offset >= a.page_size) {
+            w.offset -= a.page_size;
+            ++w.index;
+          }
+          look(w);
+        };
+        Walk kw;
+        kw.key = it.tile0 * kKeys + key0;
+        kw.index = kw.key / a.page_size;
+        kw.offset = kw.key - kw.index * a.page_size;
+        look(kw);
+        Walk vw = kw;
         // Q: rows (token, head) of this kv head's group
         wait(&sm.q_empty, q_phase ^ 1u, 0);
         q_phase ^= 1u;
@@ -878,35 +877,42 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           ptx::mbar_arrive_expect_tx(&sm.q_full, dual ? 2 * bytes : bytes);
           for (int t = 0; t < (dual ? 2 : 1); ++t)
             for (int h = 0; h < Sh::kHalves; ++h)
-              ptx::tma_load_3d(smem + Sh::kQ + t * Sh::kTileBytes + h * Sh::kSubBytes, &map_q, &sm.q_full, h * 64,
+              ptx::tma_load_3d(smem + Sh::kQ + t * Sh::kQBytes + h * Sh::kQSub, &map_q, &sm.q_full, h * 64,
                                it.head * group, it.q_tok + t * tile_tokens);
         }
         __syncwarp();
-        for (int p = 0; p < n + ahead; ++p, ++count) {
-          const uint32_t stage = stage_of(count);
+        for (int p = 0; p < n + ahead; ++p, next_stage()) {
           const bool has_k = p < n, has_v = p >= ahead;
-          const int next = page_of(p + 1);  // read ahead of its use
           if (has_k) {
             // which keys lie in a page that exists, for the softmax; published by the pair's barrier
             const uint32_t per_box = box_tokens / 8;
             uint32_t bits = 0;
-            if (loads && my_half == 0 && page < a.num_pages) bits = ((1u << per_box) - 1u) << (my_box * per_box);
+            if (loads && my_half == 0 && kw.page < a.num_pages) bits = ((1u << per_box) - 1u) << (my_box * per_box);
             bits = __reduce_or_sync(0xffffffffu, bits);
             if (lane == 0) sm.valid[(k_count + p) & (kMaskRing - 1)] = bits;
           }
-          wait(&sm.pair_empty[stage], phase_of(count) ^ 1u, 0);
+          wait(&sm.pair_empty[stage], phase ^ 1u, 0);
           if (!dead) {
             if (lane == 0) ptx::mbar_arrive_expect_tx(&sm.pair_full[stage], (has_k + has_v) * Sh::kTileBytes);
             __syncwarp();
             if (loads) {
-              if (has_v) load(&map_v, stage, 0, p - ahead, behind[ahead - 1]);
-              if (has_k) load(&map_k, stage, 1, p, page);
+              uint8_t* dst = smem + Sh::kRing + stage * Sh::kPairBytes + my_half * Sh::kSub + key0 * 128;
+              if (once) {
+                if (has_v)
+                  ptx::tma_load_4d_hint(dst, &map_v, &sm.pair_full[stage], my_half * 64, it.head, vw.offset, vw.page, policy);
+                if (has_k)
+                  ptx::tma_load_4d_hint(dst + Sh::kTileBytes, &map_k, &sm.pair_full[stage], my_half * 64, it.head, kw.offset,
+                                        kw.page, policy);
+              } else {
+                if (has_v) ptx::tma_load_4d(dst, &map_v, &sm.pair_full[stage], my_half * 64, it.head, vw.offset, vw.page);
+                if (has_k)
+                  ptx::tma_load_4d(dst + Sh::kTileBytes, &map_k, &sm.pair_full[stage], my_half * 64, it.head, kw.offset, kw.page);
+              }
             }
           }
           __syncwarp();
-          behind[1] = behind[0];
-          behind[0] = page;
-          page = next;
+          if (has_k) forward(kw);
+          if (has_v) forward(vw);
         }
         k_count += n;
       }
@@ -920,39 +926,37 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       }
     } else {
       // =============================== V guard ===============================
-      uint32_t count = 0;
       Work it;
       while (next_item(it, 3)) {
         const int n = it.tile1 - it.tile0;
-        const int ahead = it.n_tok > tile_tokens ? 1 : 2;
+        const int ahead = it.n_tok > tile_tokens ? 2 : 4;
         const int kv_len = it.pos0 + it.n_tok;
         uint32_t* special = sm.special[slot];
-        for (int p = 0; n > 0 && p < n + ahead; ++p, ++count) {
-          const uint32_t stage = stage_of(count);
-          wait(&sm.pair_full[stage], phase_of(count), 3);
+        for (int p = 0; n > 0 && p < n + ahead; ++p, next_stage()) {
+          wait(&sm.pair_full[stage], phase, 3);
           // (a pair without a V tile: nothing lies at or behind hid)
-          const int t0 = p < ahead ? -0x40000000 : (it.tile0 + p - ahead) * kTile;
+          const int t0 = p < ahead ? -0x40000000 : (it.tile0 + p - ahead) * kKeys;
           uint8_t* tile = smem + Sh::kRing + stage * Sh::kPairBytes;
           // rows behind the context: zeros (whole rows, so the swizzle does not matter)
-          const int end = min(max(kv_len - t0, 0), kTile);
+          const int end = min(max(kv_len - t0, 0), kKeys);
           // rows that some row of the block does not see: no infinities, no NaN
           const int hid = min(max(it.pos0 + 1 - t0, 0), end);
-          if (hid < kTile) {
+          if (hid < kKeys) {
             constexpr int kChunks = D / 8, kAhead = 4;  // loads under way per lane
-            for (int k0 = hid * kChunks + lane; k0 < kTile * kChunks; k0 += 32 * kAhead) {
+            for (int k0 = hid * kChunks + lane; k0 < kKeys * kChunks; k0 += 32 * kAhead) {
               uint4 v[kAhead];
 #pragma unroll
               for (int u = 0; u < kAhead; ++u) {
-                const int k = min(k0 + 32 * u, kTile * kChunks - 1);
+                const int k = min(k0 + 32 * u, kKeys * kChunks - 1);
                 const int r = k / kChunks, c = k - r * kChunks;
-                v[u] = *reinterpret_cast<const uint4*>(tile + (c >> 3) * Sh::kSubBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+                v[u] = *reinterpret_cast<const uint4*>(tile + (c >> 3) * Sh::kSub + r * 128 + (((c & 7) ^ (r & 7)) << 4));
               }
 #pragma unroll
               for (int u = 0; u < kAhead; ++u) {
                 const int k = k0 + 32 * u;
-                if (k >= kTile * kChunks) break;
+                if (k >= kKeys * kChunks) break;
                 const int r = k / kChunks, c = k - r * kChunks;
-                uint4* p = reinterpret_cast<uint4*>(tile + (c >> 3) * Sh::kSubBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+                uint4* p = reinterpret_cast<uint4*>(tile + (c >> 3) * Sh::kSub + r * 128 + (((c & 7) ^ (r & 7)) << 4));
                 if (r >= end) {
                   *p = make_uint4(0, 0, 0, 0);
                 } else if (any_nonfinite(v[u])) {
@@ -1063,7 +1067,7 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_attention_merge_kernel(co
 }
 
 int box_tokens_of(int page_size) {
-  for (int b = 128; b >= 8; b >>= 1)
+  for (int b = kKeys; b >= 8; b >>= 1)
     if (page_size % b == 0) return b;
   return 0;
 }
