@@ -52,16 +52,19 @@ __device__ int g_ca_status = 0;
 // and merged by a second launch, which spreads the rows over all SMs (the last part's CTA merging alone
 // was measured too: 5 us more per prefill, and far slower where one unit has dozens of parts).
 constexpr int kOverheadTokens = 256;
+// Length per key of a block of two score tiles and of one.  Alone on the chip the one takes 1.05 us per kv
+// tile (bound by the softmax), the other 0.7 us (bound by HBM); a mixed batch of 64 sequences took 285 us at 3 : 2,
+// 297 us at 2 : 1, 320 us at 1 : 1.
+constexpr int kTwoTiles = 3, kOneTile = 2;
 
 struct Line {
   long long total, share;
 };
 
 __device__ __forceinline__ long long unit_base(const Seq& s) { return max(s.len - s.n, 0) + kOverheadTokens; }
-// A block of more than one score tile takes twice the time per key (measured 2.3 us and 1.2 us per kv
-// tile); only the last block of a sequence can be the smaller kind.
+// Only the last block of a sequence can be one of a single score tile.
 __device__ __forceinline__ int unit_weight(const Args& a, const Seq& s, int block) {
-  return s.n - block * a.block_tokens > a.block_tokens / 2 ? 2 : 1;
+  return s.n - block * a.block_tokens > a.block_tokens / 2 ? kTwoTiles : kOneTile;
 }
 __device__ __forceinline__ long long unit_length(const Args& a, const Seq& s, int block) {
   return unit_weight(a, s, block) * (unit_base(s) + static_cast<long long>(a.block_tokens) * (block + 1));
@@ -70,7 +73,7 @@ __device__ __forceinline__ long long unit_length(const Args& a, const Seq& s, in
 __device__ __forceinline__ long long blocks_length(const Args& a, const Seq& s, long long m) {
   if (m <= 0) return 0;
   const long long k = m - 1;  // blocks of two tiles, then one of either kind
-  return 2 * (k * unit_base(s) + a.block_tokens * (k * (k + 1) / 2)) + unit_length(a, s, static_cast<int>(k));
+  return kTwoTiles * (k * unit_base(s) + a.block_tokens * (k * (k + 1) / 2)) + unit_length(a, s, static_cast<int>(k));
 }
 
 struct Unit {
@@ -93,7 +96,8 @@ __device__ __forceinline__ int cut_tile(const Unit& u, long long x, long long sh
   if (x <= 0) return 0;
   if (x >= u.length) return u.tiles;
   // Short shares (small batches): parts of eight tiles, or the merge costs more than the parts save.
-  const int grain = share >= 4096 ? 1 : 8, least = share >= 4096 ? 3 : 8;
+  const bool is_short = share < 4096 * kOneTile;
+  const int grain = is_short ? 8 : 1, least = is_short ? 8 : 3;
   // fp32 with each operation rounded by itself: cheaper than a 64-bit division, the same in both
   // kernels, and it never decreases in x
   int k = min(static_cast<int>(__fdiv_rn(__fmul_rn(static_cast<float>(x), static_cast<float>(u.tiles)),
@@ -263,34 +267,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return v;
 }
 
-// 2^x of a pair without the special-function unit, for x <= 64: x = n + f with |f| <= 1/2 (adding
-// 1.5 * 2^23 rounds to an integer in the low mantissa bits), a polynomial of degree 4 in f (relative
-// minimax on [-1/2, 1/2]: 2.6e-6, a hundredth of the fp16 rounding that follows), n added to the
-// exponent.  Below -126 the result stays near 2^-126, which rounds to 0.  NaN and inf: the caller's.
-__device__ __forceinline__ void ex2_poly(uint64_t x2, float& ya, float& yb) {
-  constexpr float kRound = 12582912.f;
-  float xa, xb;
-  split(x2, xa, xb);
-  x2 = pair(fmaxf(xa, -126.f), fmaxf(xb, -126.f));
-  const uint64_t t2 = add2(x2, pair(kRound, kRound));
-  const uint64_t n2 = add2(t2, pair(-kRound, -kRound));
-  const uint64_t f2 = fma2(n2, pair(-1.f, -1.f), x2);
-  uint64_t p2 = pair(0.009570102207362652f, 0.009570102207362652f);
-  p2 = fma2(p2, f2, pair(0.05591785907745361f, 0.05591785907745361f));
-  p2 = fma2(p2, f2, pair(0.240247443318367f, 0.240247443318367f));
-  p2 = fma2(p2, f2, pair(0.6931217908859253f, 0.6931217908859253f));
-  p2 = fma2(p2, f2, pair(0.9999992847442627f, 0.9999992847442627f));
-  float ta, tb;
-  split(t2, ta, tb);
-  split(p2, ya, yb);
-  ya = __uint_as_float((__float_as_uint(ta) << 23) + __float_as_uint(ya));
-  yb = __uint_as_float((__float_as_uint(tb) << 23) + __float_as_uint(yb));
-}
-
-// Of every 8 pairs of exponentials this many are taken by the polynomial: the special-function unit alone
-// needs as long for a score tile as the tensor core for both products.
-constexpr int kPolyPairs = 0;
-
 // Special positions of one channel: three 10-bit fields (+inf, -inf, NaN), the first position
 // minus `base`, 1023 = never.  base = the block's first hidden position, and a block spans at most
 // 256 tokens, so offsets fit.
@@ -455,7 +431,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 
   if (warp < static_cast<int>(kSoftmaxWarps)) {
     // =============================== softmax ===============================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int t = warp >> 2;                    // score tile
     const int row = (warp & 3) * 32 + lane;     // row of the tile = TMEM lane
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -500,14 +476,10 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         s_phase ^= 1u << b;
         ptx::tcgen05_fence_after();
       };
-      auto load_scores = [&](int b, uint32_t (&s)[2][32]) {
-        ptx::tmem_ld_32x32b_x32(s_col + b * kKeys, s[0]);
-        ptx::tmem_ld_32x32b_x32(s_col + b * kKeys + 32, s[1]);
-      };
+      uint32_t ok = 0;  // groups of eight keys of the tile that lie in a page that exists
       // Tile i, whose scores are in s; leaves those of the next tile there.
       auto step = [&](int i, uint32_t (&s)[2][32]) {
         const int b = i & 1;
-        const uint32_t ok = sm.valid[(k_count + off / kKeys) & (kMaskRing - 1)];
         if (ok != 0xffu || warp_pos - off < kKeys - 1) {
           const int last_col = row_pos - off;  // last visible key of the tile
 #pragma unroll
@@ -534,13 +506,9 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             const int g = c >> 4, k = 2 * (c & 15);
             const uint64_t x2 = fma2(pair(__uint_as_float(s[g][k]), __uint_as_float(s[g][k + 1])), scale2, shift2);
             float p0, p1;
-            if ((c & 7) < kPolyPairs) {
-              ex2_poly(x2, p0, p1);
-            } else {
-              split(x2, p0, p1);
-              p0 = ex2(p0);
-              p1 = ex2(p1);
-            }
+            split(x2, p0, p1);
+            p0 = ex2(p0);
+            p1 = ex2(p1);
             sum2[c & 1] = add2(sum2[c & 1], pair(p0, p1));
             p[c] = f2_to_h2(p0, p1);
           }
@@ -586,17 +554,21 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           }
           exponentials(0, 16);
         }
+        // Half by half the probabilities go to TMEM and the next tile's scores come from there meanwhile (they
+        // were issued behind the product before this tile's, so waiting for them first holds nothing up).
+        const bool more = i + 1 < steps;
+        ptx::tmem_st_32x32b_x16(s_col + b * kKeys, p);
+        if (more) {
+          await_scores(b ^ 1);
+          ptx::tmem_ld_32x32b_x32(s_col + (b ^ 1) * kKeys, s[0]);
+          ok = sm.valid[(k_count + off / kKeys) & (kMaskRing - 1)];
+        }
         exponentials(16, 32);
+        if (more) ptx::tmem_ld_32x32b_x32(s_col + (b ^ 1) * kKeys + 32, s[1]);
+        ptx::tmem_st_32x32b_x16(s_col + b * kKeys + 16, p + 16);
         float x, y;
         split(add2(sum2[0], sum2[1]), x, y);
         l += x + y;
-        // The next scores are on their way while the probabilities are stored (they were issued behind the
-        // product before this tile's, so waiting for them first holds nothing up).
-        if (i + 1 < steps) {
-          await_scores(b ^ 1);
-          load_scores(b ^ 1, s);
-        }
-        ptx::tmem_st_32x32b_x32(s_col + b * kKeys, p);
         ptx::tmem_st_wait();
         ptx::tcgen05_fence_before();
         __syncwarp();
@@ -611,7 +583,9 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       } else if (steps > 0) {
         uint32_t s[2][32];
         await_scores(0);
-        load_scores(0, s);
+        ptx::tmem_ld_32x32b_x32(s_col, s[0]);
+        ptx::tmem_ld_32x32b_x32(s_col + 32, s[1]);
+        ok = sm.valid[(k_count + off / kKeys) & (kMaskRing - 1)];
         ptx::tmem_ld_wait();
 #pragma unroll 1
         for (int i = 0; i < steps; ++i) step(i, s);
@@ -707,7 +681,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       release_item();
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 152;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     if (warp == kMmaWarp || warp == kMmaWarp + 1) {
       // =============================== MMA issue ===============================
       constexpr uint32_t idesc_qk = ptx::make_f16_idesc(kRows, kKeys);
