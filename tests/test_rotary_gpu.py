@@ -124,6 +124,22 @@ def test_rotary_of_views(ops, interleaved, pad):
     check_rotary(k, ok, pos, cos, sin, interleaved)
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("tokens,hq,hkv,dim,rot,dtype", [
+    (701, 28, 5, 128, 128, torch.float16), (5003, 31, 8, 128, 64, torch.float32), (9001, 15, 2, 80, 48, torch.float16),
+    (4500, 33, 0, 136, 72, torch.float32)])
+def test_rotary_of_many_tokens(ops, interleaved, tokens, hq, hkv, dim, rot, dtype):
+    """Several heads per thread, head counts that do not divide by it, packed views, bad positions."""
+    buf = torch.randn(tokens, (hq + hkv) * dim + 8, device=DEV).half()
+    q = buf[:, :hq * dim].view(tokens, hq, dim)
+    k = buf[:, hq * dim:(hq + hkv) * dim].view(tokens, hkv, dim)
+    cos, sin = torch.randn(300, rot // 2, device=DEV).to(dtype), torch.randn(300, rot // 2, device=DEV).to(dtype)
+    pos = torch.randint(-3, 303, (tokens,), device=DEV, dtype=torch.int32)
+    oq, ok = ops.rotary(q, k, pos, cos, sin, interleaved)
+    check_rotary(q, oq, pos, cos, sin, interleaved)
+    check_rotary(k, ok, pos, cos, sin, interleaved)
+
+
 def test_rotary_zero_sizes_and_one_row_table(ops):
     cos = torch.ones(1, 8, device=DEV).half()
     for tokens, hq, hkv in ((0, 4, 2), (3, 0, 2), (3, 4, 0)):
