@@ -1,5 +1,5 @@
 // Attention of chunks of new tokens over the paged KV cache on the 5th-generation tensor cores:
-// head_dim 64 or 128, caches [pages, P, Hkv, D] with P a multiple of 8, up to 128 query heads per kv head.
+// head_dim 64 or 128, caches of either layout with P a multiple of 8, up to 128 query heads per kv head.
 //
 // One persistent CTA per SM takes an equal share of the batch's work (below) and computes two 128-row
 // score tiles at a time:  S_t = Q_t K^T and O_t += P_t V, t = 0, 1, both accumulators in TMEM (2 x 128 columns for
@@ -200,13 +200,23 @@ __device__ __forceinline__ int part_of(const Unit& u, int c, long long share) {
   return lo >= hi ? -1 : (lo > 0 ? 2 * c : 2 * c + 1);
 }
 
-template <int D>
+// Q and, from caches [pages, P, Hkv, D], the kv tiles lie in shared memory as sub-tiles of 64 channels with
+// the 128-byte swizzle; from caches [pages, Hkv * D / 16, P, 16], whose rows of a kv head are 16 channels, the
+// kv tiles are sub-tiles of 16 channels with the 32-byte swizzle.
+template <int D, bool NZ>
 struct Shape {
-  static constexpr int kHalves = D / 64;                    // 64-channel sub-tiles
+  static constexpr int kHalves = D / 64;                    // 64-channel sub-tiles of Q
   static constexpr int kQSub = kRows * 128;                 // [128 rows][64 halfs]
   static constexpr int kQBytes = kHalves * kQSub;
-  static constexpr int kSub = kKeys * 128;                  // [64 keys][64 halfs]
-  static constexpr int kTileBytes = kHalves * kSub;         // one K or V tile
+  static constexpr int kPieces = NZ ? D / 16 : D / 64;      // sub-tiles of a kv tile
+  static constexpr int kRowBytes = NZ ? 32 : 128;
+  static constexpr int kSub = kKeys * kRowBytes;            // [64 keys][16 or 64 halfs]
+  static constexpr int kTileBytes = kPieces * kSub;         // one K or V tile
+  // Byte of the tile at which 16-byte chunk c of key r is.
+  __device__ static int chunk(int r, int c) {
+    return NZ ? (c >> 1) * kSub + r * 32 + (((c ^ (r >> 2)) & 1) << 4)
+              : (c >> 3) * kSub + r * 128 + (((c ^ r) & 7) << 4);
+  }
   static constexpr int kPairBytes = 2 * kTileBytes;         // a V tile, then the K tile that goes with it
   static constexpr int kStages = D == 128 ? 5 : 10;         // pairs in the ring
   static constexpr int kQ = 0;
@@ -232,8 +242,8 @@ struct Meta {
   uint32_t special[2][128];      // per item slot and channel: packed positions, see guard
 };
 
-template <int D>
-constexpr size_t smem_bytes() { return Shape<D>::kMeta + sizeof(Meta); }
+template <int D>  // the same for both layouts
+constexpr size_t smem_bytes() { return Shape<D, false>::kMeta + sizeof(Meta); }
 static_assert(smem_bytes<128>() <= 232448 && smem_bytes<64>() <= 232448, "shared memory");
 
 __device__ __forceinline__ float ex2(float x) {
@@ -331,11 +341,11 @@ __device__ __forceinline__ void store_row(__half* p, const float (&v)[32], float
   }
 }
 
-template <int D>
+template <int D, bool NZ>
 __global__ void __launch_bounds__(kThreads, 1)
 chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                           const __grid_constant__ CUtensorMap map_v, const Args a, const int box_tokens) {
-  using Sh = Shape<D>;
+  using Sh = Shape<D, NZ>;
   constexpr int kStages = Sh::kStages;
   extern __shared__ __align__(1024) uint8_t smem[];
   Meta& sm = *reinterpret_cast<Meta*>(smem + Sh::kMeta);
@@ -692,8 +702,9 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       // short -- one wait per pair of tiles, one per half -- and uniform over the warp (lengths broadcast, one
       // elected lane issues), because MMA descriptors come from uniform registers.
       const int t = warp - kMmaWarp;
-      const uint64_t v_desc = ptx::make_sw128_mnmajor_desc(ptx::smem_u32(smem + Sh::kRing), Sh::kSub);
-      const uint64_t k_desc = ptx::make_sw128_kmajor_desc(ptx::smem_u32(smem + Sh::kRing + Sh::kTileBytes));
+      const uint32_t v_ring = ptx::smem_u32(smem + Sh::kRing), k_ring = v_ring + Sh::kTileBytes;
+      const uint64_t v_desc = NZ ? ptx::make_sw32_desc(v_ring, Sh::kSub) : ptx::make_sw128_mnmajor_desc(v_ring, Sh::kSub);
+      const uint64_t k_desc = NZ ? ptx::make_sw32_desc(k_ring) : ptx::make_sw128_kmajor_desc(k_ring);
       const uint32_t utmem = __shfl_sync(0xffffffffu, tmem, 0);
       const uint32_t s_tmem = utmem + t * 2 * kKeys, o_tmem = utmem + 4 * kKeys + t * D;
       uint32_t q_phase = 0, p_phase = 0;  // p_phase: a bit per buffer
@@ -735,7 +746,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
               const uint64_t v = v_desc + (stage * Sh::kPairBytes >> 4);
 #pragma unroll
               for (int k = 0; k < kKeys / 16; ++k)
-                ptx::umma_f16_ts(o_tmem, s_tmem + b * kKeys + k * 8, v + (k * 2048 >> 4), idesc_pv,
+                ptx::umma_f16_ts(o_tmem, s_tmem + b * kKeys + k * 8, v + (k * 16 * Sh::kRowBytes >> 4), idesc_pv,
                                  p >= ahead + every || k > 0);
             }
             if (p < n) {  // S_t = Q_t K^T
@@ -743,7 +754,8 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 #pragma unroll
               for (int ks = 0; ks < D / 16; ++ks)
                 ptx::umma_f16(s_tmem + b * kKeys, q_desc + (((ks >> 2) * Sh::kQSub + (ks & 3) * 32) >> 4),
-                              k + (((ks >> 2) * Sh::kSub + (ks & 3) * 32) >> 4), idesc_qk, ks > 0);
+                              k + ((NZ ? ks * Sh::kSub : (ks >> 2) * Sh::kSub + (ks & 3) * 32) >> 4), idesc_qk,
+                              ks > 0);
               ptx::umma_commit(&sm.s_full[t][b]);
             }
             ptx::umma_commit(&sm.pair_empty[stage]);
@@ -757,8 +769,8 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       }
     } else if (warp == kProducerWarp) {
       // =============================== loads ===============================
-      const int boxes = kKeys / box_tokens;  // per 64-channel sub-tile
-      const int my_box = lane / Sh::kHalves, my_half = lane - my_box * Sh::kHalves;
+      const int boxes = kKeys / box_tokens;  // per sub-tile; a lane loads one box of one sub-tile
+      const int my_box = lane / Sh::kPieces, my_piece = lane - my_box * Sh::kPieces;
       const bool loads = my_box < boxes;
       const int key0 = my_box * box_tokens;  // of this lane's box in the tile
       const int skip_pages = kKeys / a.page_size, skip_keys = kKeys % a.page_size;
@@ -861,7 +873,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             // which keys lie in a page that exists, for the softmax; published by the pair's barrier
             const uint32_t per_box = box_tokens / 8;
             uint32_t bits = 0;
-            if (loads && my_half == 0 && kw.page < a.num_pages) bits = ((1u << per_box) - 1u) << (my_box * per_box);
+            if (loads && my_piece == 0 && kw.page < a.num_pages) bits = ((1u << per_box) - 1u) << (my_box * per_box);
             bits = __reduce_or_sync(0xffffffffu, bits);
             if (lane == 0) sm.valid[(k_count + p) & (kMaskRing - 1)] = bits;
           }
@@ -870,18 +882,17 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             if (lane == 0) ptx::mbar_arrive_expect_tx(&sm.pair_full[stage], (has_k + has_v) * Sh::kTileBytes);
             __syncwarp();
             if (loads) {
-              uint8_t* dst = smem + Sh::kRing + stage * Sh::kPairBytes + my_half * Sh::kSub + key0 * 128;
-              if (once) {
-                if (has_v)
-                  ptx::tma_load_4d_hint(dst, &map_v, &sm.pair_full[stage], my_half * 64, it.head, vw.offset, vw.page, policy);
-                if (has_k)
-                  ptx::tma_load_4d_hint(dst + Sh::kTileBytes, &map_k, &sm.pair_full[stage], my_half * 64, it.head, kw.offset,
-                                        kw.page, policy);
-              } else {
-                if (has_v) ptx::tma_load_4d(dst, &map_v, &sm.pair_full[stage], my_half * 64, it.head, vw.offset, vw.page);
-                if (has_k)
-                  ptx::tma_load_4d(dst + Sh::kTileBytes, &map_k, &sm.pair_full[stage], my_half * 64, it.head, kw.offset, kw.page);
-              }
+              uint8_t* dst = smem + Sh::kRing + stage * Sh::kPairBytes + my_piece * Sh::kSub + key0 * Sh::kRowBytes;
+              const int c0 = NZ ? 0 : my_piece * 64, c2 = it.head * Sh::kPieces + my_piece;
+              auto load = [&](uint8_t* to, const CUtensorMap* map, const Walk& w) {
+                const int x1 = NZ ? w.offset : it.head, x2 = NZ ? c2 : w.offset;
+                if (once)
+                  ptx::tma_load_4d_hint(to, map, &sm.pair_full[stage], c0, x1, x2, w.page, policy);
+                else
+                  ptx::tma_load_4d(to, map, &sm.pair_full[stage], c0, x1, x2, w.page);
+              };
+              if (has_v) load(dst, &map_v, vw);
+              if (has_k) load(dst + Sh::kTileBytes, &map_k, kw);
             }
           }
           __syncwarp();
@@ -923,14 +934,14 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
               for (int u = 0; u < kAhead; ++u) {
                 const int k = min(k0 + 32 * u, kKeys * kChunks - 1);
                 const int r = k / kChunks, c = k - r * kChunks;
-                v[u] = *reinterpret_cast<const uint4*>(tile + (c >> 3) * Sh::kSub + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+                v[u] = *reinterpret_cast<const uint4*>(tile + Sh::chunk(r, c));
               }
 #pragma unroll
               for (int u = 0; u < kAhead; ++u) {
                 const int k = k0 + 32 * u;
                 if (k >= kKeys * kChunks) break;
                 const int r = k / kChunks, c = k - r * kChunks;
-                uint4* p = reinterpret_cast<uint4*>(tile + (c >> 3) * Sh::kSub + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+                uint4* p = reinterpret_cast<uint4*>(tile + Sh::chunk(r, c));
                 if (r >= end) {
                   *p = make_uint4(0, 0, 0, 0);
                 } else if (any_nonfinite(v[u])) {
@@ -1040,13 +1051,13 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_attention_merge_kernel(co
   }
 }
 
-int box_tokens_of(int page_size) {
+int box_tokens_of(int64_t page_size) {
   for (int b = kKeys; b >= 8; b >>= 1)
     if (page_size % b == 0) return b;
   return 0;
 }
 
-template <int D>
+template <int D, bool NZ>
 int launch_tc_d(const Args& a, cudaStream_t st) {
   CUtensorMap mq, mk, mv;
   const uint64_t e = 2;
@@ -1059,16 +1070,18 @@ int launch_tc_d(const Args& a, cudaStream_t st) {
     if (rc != B200OPS_OK) return rc;
   }
   {
-    const uint64_t hkv = a.num_kv_heads, page = a.page_size;
-    const uint64_t dims[4] = {static_cast<uint64_t>(D), hkv, page, static_cast<uint64_t>(a.num_pages)};
-    const uint64_t strides[3] = {D * e, hkv * D * e, page * hkv * D * e};
-    const uint32_t b[4] = {64, 1, static_cast<uint32_t>(box), 1};
-    int rc = encode_f16_map(&mk, a.k_cache, 4, dims, strides, b, "chunked_paged_attention(key_cache)");
+    const uint64_t hkv = a.num_kv_heads, page = a.page_size, pages = static_cast<uint64_t>(a.num_pages);
+    const uint64_t groups = hkv * D / 16;  // of 16 channels
+    const uint64_t dims[2][4] = {{static_cast<uint64_t>(D), hkv, page, pages}, {16, page, groups, pages}};
+    const uint64_t strides[2][3] = {{D * e, hkv * D * e, page * hkv * D * e}, {16 * e, page * 16 * e, page * hkv * D * e}};
+    const uint32_t rows = static_cast<uint32_t>(box), b[2][4] = {{64, 1, rows, 1}, {16, rows, 1, 1}};
+    const CUtensorMapSwizzle swizzle = NZ ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_128B;
+    int rc = encode_f16_map(&mk, a.k_cache, 4, dims[NZ], strides[NZ], b[NZ], "chunked_paged_attention(key_cache)", swizzle);
     if (rc != B200OPS_OK) return rc;
-    rc = encode_f16_map(&mv, a.v_cache, 4, dims, strides, b, "chunked_paged_attention(value_cache)");
+    rc = encode_f16_map(&mv, a.v_cache, 4, dims[NZ], strides[NZ], b[NZ], "chunked_paged_attention(value_cache)", swizzle);
     if (rc != B200OPS_OK) return rc;
   }
-  auto kern = chunk_attention_tc_kernel<D>;
+  auto kern = chunk_attention_tc_kernel<D, NZ>;
   static std::atomic<bool> attr_set[64];
   int dev = 0;
   B200OPS_CUDA(cudaGetDevice(&dev));
@@ -1090,11 +1103,14 @@ int launch_tc_d(const Args& a, cudaStream_t st) {
 size_t cut_list_bytes(int shares) { return static_cast<size_t>(shares) * sizeof(CutUnit); }
 
 bool tc_supported(int64_t head_dim, int64_t group, int64_t page_size, int layout) {
-  return (head_dim == 64 || head_dim == 128) && group <= 128 && page_size % 8 == 0 && layout == B200OPS_KV_LAYOUT_NHD;
+  if ((head_dim != 64 && head_dim != 128) || group > 128 || page_size % 8 != 0) return false;
+  // a kv tile is loaded by at most one box per lane
+  return layout == B200OPS_KV_LAYOUT_NHD || kKeys / box_tokens_of(page_size) * (head_dim / 16) <= 32;
 }
 
 int launch_tc(const Args& a, cudaStream_t st) {
-  return a.head_dim == 64 ? launch_tc_d<64>(a, st) : launch_tc_d<128>(a, st);
+  if (a.layout == B200OPS_KV_LAYOUT_NZ) return a.head_dim == 64 ? launch_tc_d<64, true>(a, st) : launch_tc_d<128, true>(a, st);
+  return a.head_dim == 64 ? launch_tc_d<64, false>(a, st) : launch_tc_d<128, false>(a, st);
 }
 
 int status_take() {

@@ -387,6 +387,18 @@ __device__ __forceinline__ uint64_t make_sw128_mnmajor_desc(uint32_t smem_addr, 
   return d;
 }
 
+// The same two kinds of operand stored as rows of 16 halfs (32 B) with the 32-byte swizzle: a K-major
+// tile holds one k step (16 elements) per row; groups of 8 rows are 256 B apart.
+__device__ __forceinline__ uint64_t make_sw32_desc(uint32_t smem_addr, uint32_t mn_stride = 16) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3ffffu) >> 4);
+  d |= static_cast<uint64_t>(mn_stride >> 4) << 16;
+  d |= static_cast<uint64_t>(256 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(6) << 61;  // layout type: SWIZZLE_32B
+  return d;
+}
+
 // Instruction descriptor for kind::f16: fp16 A and B, both K-major, fp32 accumulator.
 __host__ __device__ constexpr uint32_t make_f16_idesc(uint32_t m, uint32_t n) {
   return (1u << 4)          // D format: f32
