@@ -10,8 +10,8 @@
 //   - for a block of at most 128 rows (decoding, short chunks): the even and the odd kv tiles of its range,
 //     two running softmaxes that are merged at the end.
 // Roles: warps 0-3 and 4-7 softmax of tile 0 and 1 (a thread owns a row), warps 8 and 9
-// issue the MMAs of tile 0 and 1, warp 10 walks the block table and issues the TMA loads, warp 11 guards
-// the V tiles (below).
+// issue the MMAs of tile 0 and 1, warp 10 goes through the CTA's work and announces every pair of kv tiles, warp 11
+// guards the V tiles (below), warps 12-15 walk the block table and issue the TMA loads.
 //
 // Online softmax: a row's reference maximum is only raised when the new maximum exceeds it by more
 // than 2^8 in the exponential, so the accumulator in TMEM is rescaled a few times per item instead of
@@ -32,13 +32,13 @@ namespace b200ops {
 namespace ca {
 namespace {
 
-constexpr int kThreads = 384;
+constexpr int kThreads = 512;
 constexpr int kRows = 128;  // rows of a score tile
 constexpr int kKeys = 64;   // keys of a kv tile
 constexpr int kMaskRing = 16;
-constexpr int kMmaWarp = 8, kProducerWarp = 10, kGuardWarp = 11;  // MMA: 8 and 9, one per score tile
+constexpr int kMmaWarp = 8, kPlanWarp = 10, kGuardWarp = 11, kLoadWarp = 12;  // MMA: 8 and 9, one per score tile
 constexpr uint32_t kSoftmaxWarps = 8;
-constexpr int kErrBase = 21;  // 21 producer, 22 MMA, 23 softmax, 24 guard, 25 misaligned shared memory
+constexpr int kErrBase = 21;  // 21 loads, 22 MMA, 23 softmax, 24 guard, 25 misaligned shared memory
 
 __device__ int g_ca_status = 0;
 
@@ -185,6 +185,38 @@ struct Work {
   int q_tok, n_tok, pos0, seq, head;
   int tile0, tile1;
   int part;  // record to write (see part_of); -1: the unit is whole, write the result
+  int once;  // the only block of its sequence: its keys are read once
+};
+
+// One box of keys of a tile, tile after tile: its page (num_pages: nothing there, TMA fills zeros) and its
+// place in it.
+struct Walk {
+  const int32_t* table;
+  int key, end, index, offset, page;
+  __device__ __forceinline__ Walk(const Args& a, const Work& it, int box_tokens, int box, bool active) {
+    table = a.block_tables + static_cast<size_t>(it.seq) * a.max_pages_per_seq;
+    end = active ? min(it.pos0 + it.n_tok, it.tile1 * kKeys) : 0;
+    key = it.tile0 * kKeys + box * box_tokens;
+    index = key / a.page_size;
+    offset = key - index * a.page_size;
+    look(a);
+  }
+  __device__ __forceinline__ void look(const Args& a) {
+    page = a.num_pages;
+    if (key < end) {
+      const int pg = table[index];
+      if (pg >= 0 && pg < a.num_pages) page = pg;
+    }
+  }
+  __device__ __forceinline__ void forward(const Args& a) {
+    key += kKeys;
+    offset += kKeys;
+    while (offset >= a.page_size) {
+      offset -= a.page_size;
+      ++index;
+    }
+    look(a);
+  }
 };
 
 // A cut unit, as the merge needs it; left by the CTA that has its first part (n = 0: none).
@@ -360,7 +392,8 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
         ptx::mbar_init(&sm.item_full[i], 1);
-        ptx::mbar_init(&sm.item_empty[i], kSoftmaxWarps + 3);  // and two MMA warps, the guard
+        // and two MMA warps, the guard, the loading warps that have a box
+        ptx::mbar_init(&sm.item_empty[i], kSoftmaxWarps + 3 + (kKeys / box_tokens * Sh::kPieces > 1 ? 4 : 2));
         for (int b = 0; b < 2; ++b) {
           ptx::mbar_init(&sm.s_full[i][b], 1);
           ptx::mbar_init(&sm.p_full[i][b], 4);
@@ -386,7 +419,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     ptx::tcgen05_fence_before();
   } else if (warp == kGuardWarp) {
     for (int i = lane; i < 2 * 128; i += 32) sm.special[i >> 7][i & 127] = kNoSpecial;
-  } else if (warp == kProducerWarp && lane == 0) {
+  } else if (warp == kPlanWarp && lane == 0) {
     ptx::prefetch_tensormap(&map_q);
     ptx::prefetch_tensormap(&map_k);
     ptx::prefetch_tensormap(&map_v);
@@ -441,7 +474,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 
   if (warp < static_cast<int>(kSoftmaxWarps)) {
     // =============================== softmax ===============================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     const int t = warp >> 2;                    // score tile
     const int row = (warp & 3) * 32 + lane;     // row of the tile = TMEM lane
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -767,18 +800,12 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         }
         release_item();
       }
-    } else if (warp == kProducerWarp) {
-      // =============================== loads ===============================
-      const int boxes = kKeys / box_tokens;  // per sub-tile; a lane loads one box of one sub-tile
-      const int my_box = lane / Sh::kPieces, my_piece = lane - my_box * Sh::kPieces;
-      const bool loads = my_box < boxes;
-      const int key0 = my_box * box_tokens;  // of this lane's box in the tile
-      const int skip_pages = kKeys / a.page_size, skip_keys = kKeys % a.page_size;
+    } else if (warp == kPlanWarp) {
+      // =============================== the CTA's work ===============================
       uint32_t q_phase = 0, k_count = 0;
       const long long x0 = blockIdx.x * line.share, x1 = x0 + line.share;
       CutUnit* cut = a.max_rows > 0 ? static_cast<CutUnit*>(a.cuts) + blockIdx.x : nullptr;
       bool listed = false;
-      const uint64_t policy = ptx::l2_evict_first();
       Unit u;
       bool more = sm.found.seq < a.bs;
       if (more) u = unit_at(a, sm.found, x0);
@@ -789,6 +816,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         it.pos0 = u.pos0;
         it.seq = u.seq;
         it.head = u.head;
+        it.once = u.s.blocks == 1;
         it.tile0 = cut_tile(u, x0 - u.at, line.share);
         it.tile1 = cut_tile(u, x1 - u.at, line.share);
         // a block without keys (zeros) belongs to the stretch that it starts in
@@ -822,39 +850,8 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         if (n <= 0) continue;
         const bool dual = it.n_tok > tile_tokens;
         const int ahead = dual ? 2 : 4;
-        // The only block of its sequence reads the keys once; they make room in L2 for those that other
-        // blocks read again.
-        const bool once = u.s.blocks == 1;
-        const int kv_len = it.pos0 + it.n_tok;
-        const int32_t* table = a.block_tables + static_cast<size_t>(it.seq) * a.max_pages_per_seq;
-        // This lane's box of one tile after the other: its page (num_pages: nothing there, TMA fills zeros) and
-        // its place in it.
-        struct Walk {
-          int key, index, offset, page;
-        };
-        auto look = [&](Walk& w) {
-          w.page = a.num_pages;
-          if (loads && w.key < kv_len && w.key < it.tile1 * kKeys) {
-            const int pg = table[w.index];
-            if (pg >= 0 && pg < a.num_pages) w.page = pg;
-          }
-        };
-        auto forward = [&](Walk& w) {
-          w.key += kKeys;
-          w.index += skip_pages;
-          w.offset += skip_keys;
-          if (w.offset >= a.page_size) {
-            w.offset -= a.page_size;
-            ++w.index;
-          }
-          look(w);
-        };
-        Walk kw;
-        kw.key = it.tile0 * kKeys + key0;
-        kw.index = kw.key / a.page_size;
-        kw.offset = kw.key - kw.index * a.page_size;
-        look(kw);
-        Walk vw = kw;
+        // a lane per box of keys: does its page exist?
+        Walk walk(a, it, box_tokens, lane, lane < kKeys / box_tokens);
         // Q: rows (token, head) of this kv head's group
         wait(&sm.q_empty, q_phase ^ 1u, 0);
         q_phase ^= 1u;
@@ -872,32 +869,15 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           if (has_k) {
             // which keys lie in a page that exists, for the softmax; published by the pair's barrier
             const uint32_t per_box = box_tokens / 8;
-            uint32_t bits = 0;
-            if (loads && my_piece == 0 && kw.page < a.num_pages) bits = ((1u << per_box) - 1u) << (my_box * per_box);
-            bits = __reduce_or_sync(0xffffffffu, bits);
-            if (lane == 0) sm.valid[(k_count + p) & (kMaskRing - 1)] = bits;
+            const uint32_t bits = walk.page < a.num_pages ? ((1u << per_box) - 1u) << (lane * per_box) : 0u;
+            const uint32_t all = __reduce_or_sync(0xffffffffu, bits);
+            if (lane == 0) sm.valid[(k_count + p) & (kMaskRing - 1)] = all;
+            walk.forward(a);
           }
           wait(&sm.pair_empty[stage], phase ^ 1u, 0);
-          if (!dead) {
-            if (lane == 0) ptx::mbar_arrive_expect_tx(&sm.pair_full[stage], (has_k + has_v) * Sh::kTileBytes);
-            __syncwarp();
-            if (loads) {
-              uint8_t* dst = smem + Sh::kRing + stage * Sh::kPairBytes + my_piece * Sh::kSub + key0 * Sh::kRowBytes;
-              const int c0 = NZ ? 0 : my_piece * 64, c2 = it.head * Sh::kPieces + my_piece;
-              auto load = [&](uint8_t* to, const CUtensorMap* map, const Walk& w) {
-                const int x1 = NZ ? w.offset : it.head, x2 = NZ ? c2 : w.offset;
-                if (once)
-                  ptx::tma_load_4d_hint(to, map, &sm.pair_full[stage], c0, x1, x2, w.page, policy);
-                else
-                  ptx::tma_load_4d(to, map, &sm.pair_full[stage], c0, x1, x2, w.page);
-              };
-              if (has_v) load(dst, &map_v, vw);
-              if (has_k) load(dst + Sh::kTileBytes, &map_k, kw);
-            }
-          }
+          // (bytes may arrive before they are announced: the phase ends with this arrival at the earliest)
+          if (!dead && lane == 0) ptx::mbar_arrive_expect_tx(&sm.pair_full[stage], (has_k + has_v) * Sh::kTileBytes);
           __syncwarp();
-          if (has_k) forward(kw);
-          if (has_v) forward(vw);
         }
         k_count += n;
       }
@@ -908,6 +888,44 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           sm.items[slot].n_tok = 0;
           ptx::mbar_arrive(&sm.item_full[slot]);
         }
+      }
+    } else if (warp >= kLoadWarp) {
+      // =============================== loads ===============================
+      // A warp issues the copies of its lanes one after the other, 58 clocks each whatever their size (and runs
+      // the code around them slowly), and small pages make many: hence four warps, two for K and two for V, a lane
+      // per box (with one warp for all, pages of 16 keys took 1.4 times, and 16-channel rows 2.2 times as long).
+      const int boxes = kKeys / box_tokens;  // per sub-tile
+      const bool is_v = (warp & 1) != 0;
+      const int first = (warp - kLoadWarp) >> 1, box = 2 * lane + first;  // of the tile
+      const int my_box = box / Sh::kPieces, my_piece = box - my_box * Sh::kPieces;
+      const bool loads = my_box < boxes;
+      const CUtensorMap* map = is_v ? &map_v : &map_k;
+      uint8_t* ring = smem + Sh::kRing + (is_v ? 0 : Sh::kTileBytes) + my_piece * Sh::kSub + my_box * box_tokens * Sh::kRowBytes;
+      const uint64_t policy = ptx::l2_evict_first();
+      Work it;
+      while (first < boxes * Sh::kPieces && next_item(it, 0)) {
+        const int n = it.tile1 - it.tile0;
+        const int ahead = n <= 0 ? 0 : (it.n_tok > tile_tokens ? 2 : 4);
+        Walk walk(a, it, box_tokens, my_box, loads);
+        const int c0 = NZ ? 0 : my_piece * 64, c2 = it.head * Sh::kPieces + my_piece;
+        for (int p = 0; p < n + ahead; ++p, next_stage()) {
+          // A pair without a tile for this warp is passed over; one with a tile cannot complete without it, so no
+          // phase of its barrier is missed.
+          if (is_v ? p < ahead : p >= n) continue;
+          wait(&sm.pair_empty[stage], phase ^ 1u, 0);
+          if (!dead && loads) {
+            uint8_t* dst = ring + stage * Sh::kPairBytes;
+            const int x1 = NZ ? walk.offset : it.head, x2 = NZ ? c2 : walk.offset;
+            // Keys that are read once make room in L2 for those that other blocks read again.
+            if (it.once)
+              ptx::tma_load_4d_hint(dst, map, &sm.pair_full[stage], c0, x1, x2, walk.page, policy);
+            else
+              ptx::tma_load_4d(dst, map, &sm.pair_full[stage], c0, x1, x2, walk.page);
+          }
+          __syncwarp();
+          walk.forward(a);
+        }
+        release_item();
       }
     } else {
       // =============================== V guard ===============================
