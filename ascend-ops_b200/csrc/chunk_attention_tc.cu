@@ -26,6 +26,7 @@
 #include "sm100_ptx.cuh"
 #include "tma_host.cuh"
 
+#include <algorithm>
 #include <atomic>
 
 namespace b200ops {
@@ -52,10 +53,10 @@ __device__ int g_ca_status = 0;
 // and merged by a second launch, which spreads the rows over all SMs (the last part's CTA merging alone
 // was measured too: 5 us more per prefill, and far slower where one unit has dozens of parts).
 constexpr int kOverheadTokens = 256;
-// Length per key of a block of two score tiles and of one.  Alone on the chip the one takes 1.05 us per kv
-// tile (bound by the softmax), the other 0.7 us (bound by HBM); a mixed batch of 64 sequences took 285 us at 3 : 2,
-// 297 us at 2 : 1, 320 us at 1 : 1.
-constexpr int kTwoTiles = 3, kOneTile = 2;
+// Length per key of a block of two score tiles and of one.  Alone on the chip the one takes 1.0 us per kv tile, the
+// other 0.75 us (bound by HBM, so less beside the first): a mixed batch of 64 sequences took 265 us at 2 : 1,
+// 271 us at 3 : 2, 277 us at 5 : 4.
+constexpr int kTwoTiles = 2, kOneTile = 1;
 
 struct Line {
   long long total, share;
@@ -567,11 +568,14 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           for (int c = 2; c < 32; c += 2) mx[g] = max3_nan(mx[g], __uint_as_float(s[g][c]), __uint_as_float(s[g][c - 1]));
         }
         const float top = max3_nan(max3_nan(mx[0], mx[1], __uint_as_float(s[0][31])), __uint_as_float(s[1][31]), mx[0]);
-        if (__any_sync(0xffffffffu, !(top <= limit))) {
+        // (Rows that are nobody's have scores of whatever was in shared memory, NaN included; with them here a warp
+        // took 2.5 times as long, and its CTA 1.7 times.)
+        const bool raise = valid && !(top <= limit);
+        if (__any_sync(0xffffffffu, raise)) {
           float f = 1.f;
-          if (!(top < INFINITY)) {
+          if (raise && !(top < INFINITY)) {
             l = NAN;  // a visible score is +inf or NaN: so is the softmax
-          } else if (top > limit) {
+          } else if (raise) {
             f = ex2((m - top) * scale);  // from -inf: 0
             m = top;
             limit = top + 8.f / scale;
@@ -597,18 +601,9 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           }
           exponentials(0, 16);
         }
-        // Half by half the probabilities go to TMEM and the next tile's scores come from there meanwhile (they
-        // were issued behind the product before this tile's, so waiting for them first holds nothing up).
         const bool more = i + 1 < steps;
-        ptx::tmem_st_32x32b_x16(s_col + b * kKeys, p);
-        if (more) {
-          await_scores(b ^ 1);
-          ptx::tmem_ld_32x32b_x32(s_col + (b ^ 1) * kKeys, s[0]);
-          ok = sm.valid[(k_count + off / kKeys) & (kMaskRing - 1)];
-        }
         exponentials(16, 32);
-        if (more) ptx::tmem_ld_32x32b_x32(s_col + (b ^ 1) * kKeys + 32, s[1]);
-        ptx::tmem_st_32x32b_x16(s_col + b * kKeys + 16, p + 16);
+        ptx::tmem_st_32x32b_x32(s_col + b * kKeys, p);
         float x, y;
         split(add2(sum2[0], sum2[1]), x, y);
         l += x + y;
@@ -616,6 +611,14 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         ptx::tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&sm.p_full[t][b]);
+        // (Taking the next scores before this tile's probabilities are out, to hide the way from TMEM, makes the two
+        // products wait for one another: 3 to 5 % more time.)
+        if (more) {
+          await_scores(b ^ 1);
+          ptx::tmem_ld_32x32b_x32(s_col + (b ^ 1) * kKeys, s[0]);
+          ptx::tmem_ld_32x32b_x32(s_col + (b ^ 1) * kKeys + 32, s[1]);
+          ok = sm.valid[(k_count + off / kKeys) & (kMaskRing - 1)];
+        }
         ptx::tmem_ld_wait();
       };
       if (!__any_sync(0xffffffffu, valid)) {  // no row of this warp is anybody's: its P may be anything
@@ -996,76 +999,84 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 
 // ---- merge of cut units ---------------------------------------------------------------------
 constexpr int kMergeThreads = 256;
-constexpr int kMergeRows = 4;  // rows a warp takes at once: their loads overlap
+constexpr int kMergeRows = 2;  // rows that eight lanes take at once: their loads overlap
+constexpr int kMergeCtas = 4;  // CTAs per unit at most
 
 // CTA (c, y): a share of the rows of the unit whose first part CTA c of the attention had.  Every row is
-// sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over its parts, in their order.  A chain of three L2 round
-// trips (the list, the maxima, the sums); bound by reading the records (D + 2 floats per row and part).
+// sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over its parts.  Eight lanes take two rows of a part; the four such
+// groups of a warp take four parts of the same rows, or two parts of four rows where a unit has no more (one
+// part at a time, 16 parts took 12 us more).  The groups' sums are added in a fixed order.  A chain of three
+// L2 round trips (the list, the maxima, the sums); bound by reading the records (D + 2 floats per row and part).
 template <int D>
 __global__ void __launch_bounds__(kMergeThreads) chunk_attention_merge_kernel(const Args a) {
-  constexpr int kPer = D / 32;  // channels per lane
+  constexpr int kPer = D / 32;  // times four channels per lane
   pdl_trigger();
   pdl_wait();
   const CutUnit& cut = static_cast<const CutUnit*>(a.cuts)[blockIdx.x];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n = cut.n, rows = cut.n_tok * a.group;
-  const int r0 = (blockIdx.y * (kMergeThreads / 32) + warp) * kMergeRows;
-  if (n == 0 || r0 >= rows) return;
-  float m[kMergeRows], l[kMergeRows], acc[kMergeRows][kPer];
-#pragma unroll
-  for (int j = 0; j < kMergeRows; ++j) {
-    m[j] = -INFINITY;
-    l[j] = 0.f;
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) acc[j][k] = 0.f;
-  }
-  for (int i = lane; i < n; i += 32) {
-    const float2* ml = a.part_ml + static_cast<size_t>(cut.parts[i]) * a.slot_rows;
-#pragma unroll
-    for (int j = 0; j < kMergeRows; ++j) m[j] = fmaxf(m[j], ml[min(r0 + j, rows - 1)].x);
-  }
-#pragma unroll
-  for (int j = 0; j < kMergeRows; ++j) {
-    m[j] = warp_max(m[j]);
-    if (m[j] == -INFINITY) m[j] = 0.f;
-  }
-#pragma unroll 2
-  for (int i = 0; i < n; ++i) {
-    const size_t pr = static_cast<size_t>(cut.parts[i]) * a.slot_rows;
+  if (n == 0) return;
+  const int parts = n > 2 ? 4 : 2, warp_rows = kMergeRows * 4 / parts;
+  const int sub = (lane >> 3) & (parts - 1), row = (lane >> 3) / parts * kMergeRows, channel = (lane & 7) * 4;
+  const int step = gridDim.y * (kMergeThreads / 32) * warp_rows;
+  for (int r_warp = (blockIdx.y * (kMergeThreads / 32) + warp) * warp_rows; r_warp < rows; r_warp += step) {
+    const int r0 = r_warp + row;
+    float m[kMergeRows], l[kMergeRows], acc[kMergeRows][kPer * 4];
 #pragma unroll
     for (int j = 0; j < kMergeRows; ++j) {
-      const int r = min(r0 + j, rows - 1);
-      const float2 ml = a.part_ml[pr + r];
-      const float w = exp2f(ml.x - m[j]);
-      l[j] += ml.y * w;
-      float v[kPer];
-      const float* src = a.part_o + (pr + r) * D + lane * kPer;
-      if constexpr (kPer == 4) {
-        const float4 x = *reinterpret_cast<const float4*>(src);
-        v[0] = x.x;
-        v[1] = x.y;
-        v[2] = x.z;
-        v[3] = x.w;
-      } else {
-        const float2 x = *reinterpret_cast<const float2*>(src);
-        v[0] = x.x;
-        v[1] = x.y;
-      }
+      m[j] = -INFINITY;
+      l[j] = 0.f;
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) acc[j][k] = fmaf(w, w != 0.f ? v[k] : 0.f, acc[j][k]);
+      for (int k = 0; k < kPer * 4; ++k) acc[j][k] = 0.f;
     }
-  }
+    for (int i = lane & 7; i < n; i += 8) {
+      const float2* ml = a.part_ml + static_cast<size_t>(cut.parts[i]) * a.slot_rows;
 #pragma unroll
-  for (int j = 0; j < kMergeRows; ++j) {
-    const int r = r0 + j;
-    if (r >= rows) break;
-    const float inv = l[j] == 0.f ? 0.f : 1.0f / l[j];  // nothing visible: zeros; a NaN sum stays NaN
-    const int tok = r / a.group;
-    __half* dst = a.out + (static_cast<size_t>(cut.q_tok + tok) * a.num_heads + cut.head * a.group + r - tok * a.group) * D + lane * kPer;
-    if constexpr (kPer == 4)
-      *reinterpret_cast<uint2*>(dst) = make_uint2(f2_to_h2(acc[j][0] * inv, acc[j][1] * inv), f2_to_h2(acc[j][2] * inv, acc[j][3] * inv));
-    else
-      *reinterpret_cast<uint32_t*>(dst) = f2_to_h2(acc[j][0] * inv, acc[j][1] * inv);
+      for (int j = 0; j < kMergeRows; ++j) m[j] = fmaxf(m[j], ml[min(r0 + j, rows - 1)].x);
+    }
+#pragma unroll
+    for (int j = 0; j < kMergeRows; ++j) {
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) m[j] = fmaxf(m[j], __shfl_xor_sync(0xffffffffu, m[j], o));
+      if (m[j] == -INFINITY) m[j] = 0.f;
+    }
+    for (int i = sub; i < n; i += parts) {
+      const size_t pr = static_cast<size_t>(cut.parts[i]) * a.slot_rows;
+#pragma unroll
+      for (int j = 0; j < kMergeRows; ++j) {
+        const int r = min(r0 + j, rows - 1);
+        const float2 ml = a.part_ml[pr + r];
+        const float w = exp2f(ml.x - m[j]);
+        l[j] += ml.y * w;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+          const float4 x = *reinterpret_cast<const float4*>(a.part_o + (pr + r) * D + k * 32 + channel);
+          const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[j][4 * k + e] = fmaf(w, w != 0.f ? v[e] : 0.f, acc[j][4 * k + e]);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kMergeRows; ++j) {
+#pragma unroll
+      for (int o = 8; o < 32; o <<= 1) {
+        if (o >= 8 * parts) break;
+        l[j] += __shfl_xor_sync(0xffffffffu, l[j], o);
+#pragma unroll
+        for (int k = 0; k < kPer * 4; ++k) acc[j][k] += __shfl_xor_sync(0xffffffffu, acc[j][k], o);
+      }
+      const int r = r0 + j;
+      if (r >= rows) continue;
+      const float inv = l[j] == 0.f ? 0.f : 1.0f / l[j];  // nothing visible: zeros; a NaN sum stays NaN
+      const int tok = r / a.group;
+      __half* dst = a.out + (static_cast<size_t>(cut.q_tok + tok) * a.num_heads + cut.head * a.group + r - tok * a.group) * D + channel;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k)
+        if (k % parts == sub)
+          *reinterpret_cast<uint2*>(dst + k * 32) = make_uint2(f2_to_h2(acc[j][4 * k] * inv, acc[j][4 * k + 1] * inv),
+                                                               f2_to_h2(acc[j][4 * k + 2] * inv, acc[j][4 * k + 3] * inv));
+    }
   }
 }
 
@@ -1109,9 +1120,9 @@ int launch_tc_d(const Args& a, cudaStream_t st) {
   }
   B200OPS_CUDA(launch_kernel(kern, dim3(a.shares), dim3(kThreads), smem_bytes<D>(), st, mq, mk, mv, a, box));
   if (a.max_rows > 0) {  // some context may be long enough to be cut
-    constexpr int kRowsPerCta = kMergeThreads / 32 * kMergeRows;
-    B200OPS_CUDA(launch_kernel(chunk_attention_merge_kernel<D>, dim3(a.shares, (a.slot_rows + kRowsPerCta - 1) / kRowsPerCta),
-                               dim3(kMergeThreads), 0, st, a));
+    constexpr int kRowsPerCta = kMergeThreads / 32 * 2 * kMergeRows;  // of a unit of two parts
+    const int y = std::min((a.slot_rows + kRowsPerCta - 1) / kRowsPerCta, kMergeCtas);
+    B200OPS_CUDA(launch_kernel(chunk_attention_merge_kernel<D>, dim3(a.shares, y), dim3(kMergeThreads), 0, st, a));
   }
   return B200OPS_OK;
 }
