@@ -318,3 +318,77 @@ def test_offsets_past_32_bits(ops):
              ctx=torch.tensor([370], dtype=torch.int32, device=DEV),
              starts=torch.tensor([0, 37], dtype=torch.int32, device=DEV), hkv=hkv, page=page, layout=NHD)
     check(call(ops, s), s)
+
+
+@pytest.mark.parametrize("hq,hkv,d,page", [
+    (28, 4, 128, 8), (8, 2, 128, 64), (6, 2, 64, 8), (16, 1, 64, 128), (12, 4, 128, 32), (14, 2, 128, 56), (3, 3, 64, 40)])
+@pytest.mark.parametrize("lens", [
+    [(5, 5), (1, 300), (0, 10), (17, 40), (128, 128)], [(3, 2), (1, 0), (20, 7), (2, 2)], [(300, 1700), (1, 2500)]])
+def test_caches_in_rows_of_16_channels(ops, lens, hq, hkv, d, page):
+    s = make(lens, hq, hkv, d, page, NZ, seed=hq + page)
+    check(call(ops, s), s)
+
+
+@pytest.mark.parametrize("layout", [NHD, NZ])
+@pytest.mark.parametrize("hq,hkv,d,page,lens", [
+    (14, 2, 128, 32, [(1, 700)] * 200),
+    (14, 2, 128, 128, [(400, 400)] * 6),
+    (8, 2, 64, 16, [(1, 300), (100, 260), (1, 900), (73, 800)] * 20),
+    (28, 4, 128, 128, [(1, 5), (0, 40), (36, 36), (1, 1), (19, 500), (2, 1), (18, 4000), (1, 66)] * 8)])
+def test_many_pieces_of_work_in_a_row(ops, layout, hq, hkv, d, page, lens):
+    """Every CTA goes through several items of both kinds; the same bits each time, also back to back."""
+    s = make(lens, hq, hkv, d, page, layout, seed=len(lens))
+    outs = [call(ops, s) for _ in range(4)]
+    check(outs[0], s)
+    for o in outs[1:]:
+        assert torch.equal(o, outs[0])
+
+
+@pytest.mark.parametrize("hq,hkv,d,lens", [
+    (7, 1, 128, [(1, 30000)]), (2, 2, 128, [(1, 1024), (1, 1100), (1, 1600), (1, 2100)]), (4, 1, 64, [(1, 12000), (3, 9000)]),
+    (4, 1, 128, [(200, 9000)]), (128, 1, 128, [(2, 6000)])])
+def test_contexts_cut_into_many_parts(ops, hq, hkv, d, lens):
+    s = make(lens, hq, hkv, d, 64, seed=hq)
+    check(call(ops, s), s)
+
+
+def test_non_finite_query_rows_stay_by_themselves(ops):
+    """A NaN and an infinite query: their rows are NaN, all others keep their bits."""
+    s = make([(50, 900), (1, 700)], 28, 4, 128, 128, seed=30)
+    clean = call(ops, s)
+    s["q"][7, 3, 5] = float("nan")
+    s["q"][20, 27] = float("inf")
+    got = call(ops, s)
+    assert bool(got[7, 3].isnan().all()) and bool(got[20, 27].isnan().all())
+    hit = torch.zeros(51, 28, dtype=torch.bool, device=DEV)
+    hit[7, 3] = hit[20, 27] = True
+    assert torch.equal(got[~hit], clean[~hit])
+
+
+def test_output_aligned_to_16_bytes_only(cabi):
+    s = make([(60, 500), (1, 3000), (2, 60)], 28, 4, 128, 128, seed=14)
+    raw = torch.zeros(s["q"].numel() + 16, dtype=torch.float16, device=DEV)
+    shift = 8 if raw.data_ptr() % 32 == 0 else 0
+    out = raw[shift:shift + s["q"].numel()].view(s["q"].shape)
+    assert out.data_ptr() % 32 == 16
+    ws = torch.empty(cabi.chunked_paged_attention_workspace_size(63, 3, 28, 4, 128, 128, s["table"].shape[1]),
+                     dtype=torch.uint8, device=DEV)
+    cabi.chunked_paged_attention(s["q"], s["kc"], s["vc"], s["table"], s["ctx"], s["starts"], out, 4, 128, NHD, ws)
+    check(out, s)
+
+
+def test_two_calls_at_once(ops):
+    """Two streams, each with calls of its own, at the same time on the device."""
+    a, b = make([(60, 2500), (1, 3000)], 28, 4, 128, 128, seed=15), make([(300, 300), (1, 900)], 8, 2, 64, 16, seed=16)
+    want_a, want_b = call(ops, a), call(ops, b)
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(8):
+        with torch.cuda.stream(sa):
+            outs.append((call(ops, a), want_a))
+        with torch.cuda.stream(sb):
+            outs.append((call(ops, b), want_b))
+    torch.cuda.synchronize()
+    for got, want in outs:
+        assert torch.equal(got, want)
