@@ -18,6 +18,15 @@
 // once per tile; probabilities are then up to 256, well inside fp16, and the final division
 // by the sum in fp32 makes up for any reference.
 //
+// Bounds.  With more than one score tile per block, the tensor core (a pair of tiles of 128 rows x 64 keys, D = 128: 1280
+// clocks) and the special-function unit (1024) are near each other, and what is lost is the way between them: 4096
+// new tokens at context 16384, 28 heads of 128 on 4, take 725 us = 1.16 PFLOP/s on a cool chip (60 % tensor pipe,
+// 50 % special functions active), 830 us = 1.01 PFLOP/s in a row under the power limit, where a large matrix
+// product runs at 1.4.  Keys 64 at a time with two score buffers each, because 128 at a time leave TMEM room for one (770 us).
+// Head dimension 64 has half the products for the same exponentials: 129 us for 4096 tokens, 32 heads on 8.
+// Single tokens are bound by HBM: 37 contexts of 8192 take 101 us = 6.2 TB/s; a few short ones by a chain of latencies
+// (19 us for four of 1300, of which the merge is 3).
+//
 // V tiles: a hidden key has probability 0, but 0 * inf is NaN.  Slots past the context and pages that
 // name nothing are filled with zeros (by TMA outside the tensor, by the guard warp inside a box), and
 // the non-finite values of keys that some row of the block does not see are taken out and
