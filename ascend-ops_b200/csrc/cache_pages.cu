@@ -326,6 +326,7 @@ extern "C" int b200ops_compact_pages(void* const* tensors, int64_t num_tensors, 
   if (workspace == nullptr || workspace_size < need)
     return fail(B200OPS_EWORKSPACE, "compact_pages: workspace of %zu bytes needed, got %zu", need,
                 workspace ? workspace_size : (size_t)0);
+  B200OPS_REQUIRE(aligned16(workspace), "compact_pages: the workspace must be 16-byte aligned");
   int32_t* moves = static_cast<int32_t*>(workspace);
   int32_t* move_src = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + 256);
   int32_t* move_dst = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(move_src) +

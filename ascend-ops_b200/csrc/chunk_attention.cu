@@ -446,8 +446,11 @@ void plan_shape(Args* a, bool tc) {
   a->max_rows = static_cast<int>(rows);
 }
 
-// Lays the workspace out from `base` (may be null: only the size is wanted).
+// Lays the workspace out from `base` (may be null: only the size is wanted).  Callers align it to 16 bytes, the
+// kernels' 32-byte stores need more: the parts begin at the next multiple of 256, and the size has room for that.
 size_t lay_out(Args* a, char* base) {
+  constexpr size_t kSlack = 256 - 16;
+  base = reinterpret_cast<char*>(align256(reinterpret_cast<uintptr_t>(base)));
   size_t off = 0;
   auto take = [&](size_t bytes) {
     char* p = base + off;
@@ -459,14 +462,14 @@ size_t lay_out(Args* a, char* base) {
     a->cuts = take(a->max_rows > 0 ? cut_list_bytes(a->shares) : 0);
     a->part_ml = reinterpret_cast<float2*>(take(static_cast<size_t>(a->max_rows) * sizeof(float2)));
     a->part_o = reinterpret_cast<float*>(take(static_cast<size_t>(a->max_rows) * a->head_dim * sizeof(float)));
-    return off;
+    return off + kSlack;
   }
   a->prefix = reinterpret_cast<int*>(take((static_cast<size_t>(a->bs) + 1) * sizeof(int) + static_cast<size_t>(a->bs) * sizeof(SeqPlan)));
   a->counters = reinterpret_cast<int*>(take(static_cast<size_t>(a->max_split_items) * sizeof(int)));
   a->items = reinterpret_cast<Item*>(take(static_cast<size_t>(a->max_items) * sizeof(Item)));
   a->part_ml = reinterpret_cast<float2*>(take(static_cast<size_t>(a->max_rows) * sizeof(float2)));
   a->part_o = reinterpret_cast<float*>(take(static_cast<size_t>(a->max_rows) * a->head_dim * sizeof(float)));
-  return off;
+  return off + kSlack;
 }
 
 }  // namespace

@@ -491,7 +491,8 @@ int b200ops_compact_pages(void* const* tensors, int64_t num_tensors, int64_t num
                           int32_t* num_live, void* workspace, size_t workspace_size, void* stream);
 
 /*
- * Health word of the pipelined kernels (grouped_matmul, paged_attention's TMA path).  Their
+ * Health word of the pipelined kernels (grouped_matmul, paged_attention's TMA path,
+ * chunked_paged_attention's tensor-core path).  Their
  * producer/consumer waits are bounded; a wait that runs out ends the kernel and leaves a
  * non-zero code here.  This call synchronises the device, returns the code in *status
  * (0 = healthy) and clears it.  Diagnostic only; it has no counterpart in the reference.

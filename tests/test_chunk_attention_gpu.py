@@ -392,3 +392,18 @@ def test_two_calls_at_once(ops):
     torch.cuda.synchronize()
     for got, want in outs:
         assert torch.equal(got, want)
+
+
+def test_workspace_aligned_to_16_bytes_only(cabi):
+    for seed, (hq, hkv, d, page) in enumerate([(28, 4, 128, 128), (4, 2, 32, 16)]):
+        s = make([(60, 5000), (1, 3000), (2, 60)], hq, hkv, d, page, seed=seed)
+        need = cabi.chunked_paged_attention_workspace_size(63, 3, hq, hkv, d, page, s["table"].shape[1])
+        raw = torch.full((need + 512,), 0x5C, dtype=torch.uint8, device=DEV)
+        assert raw.data_ptr() % 256 == 0
+        for at in (16, 240):
+            out = torch.empty_like(s["q"])
+            cabi.chunked_paged_attention(s["q"], s["kc"], s["vc"], s["table"], s["ctx"], s["starts"], out, hkv, page, NHD,
+                                         raw[at:at + need])
+            check(out, s)
+            assert bool((raw[:at] == 0x5C).all()) and bool((raw[at + need:] == 0x5C).all())
+            raw.fill_(0x5C)

@@ -139,3 +139,15 @@ def test_python_layer_refusals(ops):
         ops.rotary_tables(f, 4, device="cpu")
     with pytest.raises(RuntimeError, match="float64 CPU"):
         ops.rotary_tables(f.float(), 4, device="cuda:0")
+
+
+def test_workspaces_off_their_alignment_are_refused(cabi):
+    lib = cabi.load()
+    table = (ctypes.c_void_p * 1)(1 << 20)
+    need = lib.b200ops_compact_pages_workspace_size(10)
+    assert lib.b200ops_compact_pages(table, 1, 10, 64, ONE, ONE, 2, 3, ctypes.c_void_p(8192), ONE, ONE,
+                                     ctypes.c_void_p(4096 + 2), need, NULL) == cabi.EINVAL
+    assert "aligned" in cabi.last_error()
+    need = lib.b200ops_chunked_paged_attention_workspace_size(64, 2, 8, 2, 128, 16, 64)
+    assert lib.b200ops_chunked_paged_attention(ONE, ONE, ONE, ONE, ONE, ONE, ONE, 64, 2, 8, 2, 128, 100, 16, 64, 1,
+                                               ctypes.c_void_p(4096 + 8), need, NULL) == cabi.EINVAL
