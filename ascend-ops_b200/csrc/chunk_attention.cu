@@ -538,10 +538,10 @@ extern "C" size_t b200ops_chunked_paged_attention_workspace_size(int64_t num_tok
     return 0;
   ca::Args a = ca::shape_args(num_tokens, bs, num_heads, num_kv_heads, head_dim, page_size, max_pages_per_seq, false);
   size_t need = ca::lay_out(&a, nullptr);
-  if (ca::tc_supported(head_dim, num_heads / num_kv_heads, page_size, B200OPS_KV_LAYOUT_NHD)) {
+  if (ca::tc_supported(head_dim, num_heads / num_kv_heads, page_size)) {
     a = ca::shape_args(num_tokens, bs, num_heads, num_kv_heads, head_dim, page_size, max_pages_per_seq, true);
     const size_t tc = ca::lay_out(&a, nullptr);
-    if (tc > need) need = tc;  // enough for either kernel: the layout and the option are not known here
+    if (tc > need) need = tc;  // enough for either kernel: the option may change
   }
   return need;
 }
@@ -564,7 +564,7 @@ extern "C" int b200ops_chunked_paged_attention(const void* q, const void* key_ca
                   "chunked_paged_attention: null pointer");
   B200OPS_REQUIRE(aligned16(q) && aligned16(key_cache) && aligned16(value_cache) && aligned16(out),
                   "chunked_paged_attention: pointers must be 16-byte aligned");
-  const bool tc = knob(kKnobPaMode, 0) != 2 && ca::tc_supported(head_dim, num_heads / num_kv_heads, page_size, layout);
+  const bool tc = knob(kKnobPaMode, 0) != 2 && ca::tc_supported(head_dim, num_heads / num_kv_heads, page_size);
   ca::Args a = ca::shape_args(num_tokens, bs, num_heads, num_kv_heads, head_dim, page_size, max_pages_per_seq, tc);
   const size_t need = ca::lay_out(&a, static_cast<char*>(workspace));
   if (workspace == nullptr || workspace_size < need)

@@ -151,7 +151,7 @@ __device__ __forceinline__ void merge_row(const Args& a, int row0, int rows, int
 
 int launch_plan(const Args& a, cudaStream_t st);
 int launch_general(const Args& a, cudaStream_t st);
-bool tc_supported(int64_t head_dim, int64_t group, int64_t page_size, int layout);
+bool tc_supported(int64_t head_dim, int64_t group, int64_t page_size);
 int launch_tc(const Args& a, cudaStream_t st);
 size_t cut_list_bytes(int shares);
 

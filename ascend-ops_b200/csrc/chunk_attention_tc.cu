@@ -243,20 +243,22 @@ __device__ __forceinline__ int part_of(const Unit& u, int c, long long share) {
 }
 
 // Q and, from caches [pages, P, Hkv, D], the kv tiles lie in shared memory as sub-tiles of 64 channels with
-// the 128-byte swizzle; from caches [pages, Hkv * D / 16, P, 16], whose rows of a kv head are 16 channels, the
-// kv tiles are sub-tiles of 16 channels with the 32-byte swizzle.
+// the 128-byte swizzle: a copy brings `box_tokens` keys of a sub-tile.  From caches [pages, Hkv * D / 16, P, 16] a
+// copy brings all channels of 8 keys, [D / 16][8 keys][16 halfs] with the 32-byte swizzle: such pieces are the same
+// distance apart whatever the page size, as the products' descriptors need (one channel row of 16 keys per copy,
+// 32 copies a tile, took 1.5 times as long for a mixed batch on pages of 16).
 template <int D, bool NZ>
 struct Shape {
   static constexpr int kHalves = D / 64;                    // 64-channel sub-tiles of Q
   static constexpr int kQSub = kRows * 128;                 // [128 rows][64 halfs]
   static constexpr int kQBytes = kHalves * kQSub;
-  static constexpr int kPieces = NZ ? D / 16 : D / 64;      // sub-tiles of a kv tile
-  static constexpr int kRowBytes = NZ ? 32 : 128;
-  static constexpr int kSub = kKeys * kRowBytes;            // [64 keys][16 or 64 halfs]
-  static constexpr int kTileBytes = kPieces * kSub;         // one K or V tile
+  static constexpr int kPieces = NZ ? 1 : D / 64;           // copies per box of keys
+  static constexpr int kGroup = D * 16;                     // NZ: 8 keys
+  static constexpr int kSub = kKeys * 128;                  // [64 keys][64 halfs]
+  static constexpr int kTileBytes = kKeys * D * 2;          // one K or V tile
   // Byte of the tile at which 16-byte chunk c of key r is.
   __device__ static int chunk(int r, int c) {
-    return NZ ? (c >> 1) * kSub + r * 32 + (((c ^ (r >> 2)) & 1) << 4)
+    return NZ ? (r >> 3) * kGroup + (c >> 1) * 256 + (r & 7) * 32 + (((c ^ (r >> 2)) & 1) << 4)
               : (c >> 3) * kSub + r * 128 + (((c ^ r) & 7) << 4);
   }
   static constexpr int kPairBytes = 2 * kTileBytes;         // a V tile, then the K tile that goes with it
@@ -748,8 +750,8 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       // elected lane issues), because MMA descriptors come from uniform registers.
       const int t = warp - kMmaWarp;
       const uint32_t v_ring = ptx::smem_u32(smem + Sh::kRing), k_ring = v_ring + Sh::kTileBytes;
-      const uint64_t v_desc = NZ ? ptx::make_sw32_desc(v_ring, Sh::kSub) : ptx::make_sw128_mnmajor_desc(v_ring, Sh::kSub);
-      const uint64_t k_desc = NZ ? ptx::make_sw32_desc(k_ring) : ptx::make_sw128_kmajor_desc(k_ring);
+      const uint64_t v_desc = NZ ? ptx::make_sw32_desc(v_ring, Sh::kGroup, 256) : ptx::make_sw128_mnmajor_desc(v_ring, Sh::kSub);
+      const uint64_t k_desc = NZ ? ptx::make_sw32_desc(k_ring, Sh::kGroup) : ptx::make_sw128_kmajor_desc(k_ring);
       const uint32_t utmem = __shfl_sync(0xffffffffu, tmem, 0);
       const uint32_t s_tmem = utmem + t * 2 * kKeys, o_tmem = utmem + 4 * kKeys + t * D;
       uint32_t q_phase = 0, p_phase = 0;  // p_phase: a bit per buffer
@@ -791,7 +793,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
               const uint64_t v = v_desc + (stage * Sh::kPairBytes >> 4);
 #pragma unroll
               for (int k = 0; k < kKeys / 16; ++k)
-                ptx::umma_f16_ts(o_tmem, s_tmem + b * kKeys + k * 8, v + (k * 16 * Sh::kRowBytes >> 4), idesc_pv,
+                ptx::umma_f16_ts(o_tmem, s_tmem + b * kKeys + k * 8, v + (k * (NZ ? 2 * Sh::kGroup : 2048) >> 4), idesc_pv,
                                  p >= ahead + every || k > 0);
             }
             if (p < n) {  // S_t = Q_t K^T
@@ -799,7 +801,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 #pragma unroll
               for (int ks = 0; ks < D / 16; ++ks)
                 ptx::umma_f16(s_tmem + b * kKeys, q_desc + (((ks >> 2) * Sh::kQSub + (ks & 3) * 32) >> 4),
-                              k + ((NZ ? ks * Sh::kSub : (ks >> 2) * Sh::kSub + (ks & 3) * 32) >> 4), idesc_qk,
+                              k + ((NZ ? ks * 256 : (ks >> 2) * Sh::kSub + (ks & 3) * 32) >> 4), idesc_qk,
                               ks > 0);
               ptx::umma_commit(&sm.s_full[t][b]);
             }
@@ -905,21 +907,22 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       // =============================== loads ===============================
       // A warp issues the copies of its lanes one after the other, 58 clocks each whatever their size (and runs
       // the code around them slowly), and small pages make many: hence four warps, two for K and two for V, a lane
-      // per box (with one warp for all, pages of 16 keys took 1.4 times, and 16-channel rows 2.2 times as long).
-      const int boxes = kKeys / box_tokens;  // per sub-tile
+      // per copy (with one warp for all, pages of 16 keys took 1.4 times as long).
+      const int boxes = kKeys / box_tokens;
       const bool is_v = (warp & 1) != 0;
       const int first = (warp - kLoadWarp) >> 1, box = 2 * lane + first;  // of the tile
       const int my_box = box / Sh::kPieces, my_piece = box - my_box * Sh::kPieces;
       const bool loads = my_box < boxes;
       const CUtensorMap* map = is_v ? &map_v : &map_k;
-      uint8_t* ring = smem + Sh::kRing + (is_v ? 0 : Sh::kTileBytes) + my_piece * Sh::kSub + my_box * box_tokens * Sh::kRowBytes;
+      uint8_t* ring = smem + Sh::kRing + (is_v ? 0 : Sh::kTileBytes) +
+                      (NZ ? my_box * Sh::kGroup : my_piece * Sh::kSub + my_box * box_tokens * 128);
       const uint64_t policy = ptx::l2_evict_first();
       Work it;
       while (first < boxes * Sh::kPieces && next_item(it, 0)) {
         const int n = it.tile1 - it.tile0;
         const int ahead = n <= 0 ? 0 : (it.n_tok > tile_tokens ? 2 : 4);
         Walk walk(a, it, box_tokens, my_box, loads);
-        const int c0 = NZ ? 0 : my_piece * 64, c2 = it.head * Sh::kPieces + my_piece;
+        const int c0 = NZ ? 0 : my_piece * 64, c2 = it.head * (D / 16);
         for (int p = 0; p < n + ahead; ++p, next_stage()) {
           // A pair without a tile for this warp is passed over; one with a tile cannot complete without it, so no
           // phase of its barrier is missed.
@@ -1099,7 +1102,7 @@ template <int D, bool NZ>
 int launch_tc_d(const Args& a, cudaStream_t st) {
   CUtensorMap mq, mk, mv;
   const uint64_t e = 2;
-  const int box = box_tokens_of(a.page_size);
+  const int box = NZ ? 8 : box_tokens_of(a.page_size);  // keys per copy
   {
     const uint64_t dims[3] = {static_cast<uint64_t>(D), static_cast<uint64_t>(a.num_heads), static_cast<uint64_t>(a.num_tokens)};
     const uint64_t strides[2] = {D * e, static_cast<uint64_t>(a.num_heads) * D * e};
@@ -1112,7 +1115,7 @@ int launch_tc_d(const Args& a, cudaStream_t st) {
     const uint64_t groups = hkv * D / 16;  // of 16 channels
     const uint64_t dims[2][4] = {{static_cast<uint64_t>(D), hkv, page, pages}, {16, page, groups, pages}};
     const uint64_t strides[2][3] = {{D * e, hkv * D * e, page * hkv * D * e}, {16 * e, page * 16 * e, page * hkv * D * e}};
-    const uint32_t rows = static_cast<uint32_t>(box), b[2][4] = {{64, 1, rows, 1}, {16, rows, 1, 1}};
+    const uint32_t rows = static_cast<uint32_t>(box), b[2][4] = {{64, 1, rows, 1}, {16, rows, D / 16, 1}};
     const CUtensorMapSwizzle swizzle = NZ ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_128B;
     int rc = encode_f16_map(&mk, a.k_cache, 4, dims[NZ], strides[NZ], b[NZ], "chunked_paged_attention(key_cache)", swizzle);
     if (rc != B200OPS_OK) return rc;
@@ -1140,10 +1143,8 @@ int launch_tc_d(const Args& a, cudaStream_t st) {
 
 size_t cut_list_bytes(int shares) { return static_cast<size_t>(shares) * sizeof(CutUnit); }
 
-bool tc_supported(int64_t head_dim, int64_t group, int64_t page_size, int layout) {
-  if ((head_dim != 64 && head_dim != 128) || group > 128 || page_size % 8 != 0) return false;
-  // a kv tile is loaded by at most one box per lane
-  return layout == B200OPS_KV_LAYOUT_NHD || kKeys / box_tokens_of(page_size) * (head_dim / 16) <= 32;
+bool tc_supported(int64_t head_dim, int64_t group, int64_t page_size) {
+  return (head_dim == 64 || head_dim == 128) && group <= 128 && page_size % 8 == 0;
 }
 
 int launch_tc(const Args& a, cudaStream_t st) {

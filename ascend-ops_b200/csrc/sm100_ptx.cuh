@@ -378,13 +378,14 @@ __device__ __forceinline__ uint64_t make_sw128_mnmajor_desc(uint32_t smem_addr, 
   return d;
 }
 
-// The same two kinds of operand stored as rows of 16 halfs (32 B) with the 32-byte swizzle: a K-major
-// tile holds one k step (16 elements) per row; groups of 8 rows are 256 B apart.
-__device__ __forceinline__ uint64_t make_sw32_desc(uint32_t smem_addr, uint32_t mn_stride = 16) {
+// The same two kinds of operand stored as rows of 16 halfs (32 B) with the 32-byte swizzle, in blocks of 8 rows
+// (256 B).  K-major: a row is one k step (16 elements); the next 8 rows start `stride` bytes on.  Contiguous
+// along M or N: a row is 16 elements of one k; the next 8 k start `stride`, the next 16 elements `mn_stride` bytes on.
+__device__ __forceinline__ uint64_t make_sw32_desc(uint32_t smem_addr, uint32_t stride, uint32_t mn_stride = 16) {
   uint64_t d = 0;
   d |= static_cast<uint64_t>((smem_addr & 0x3ffffu) >> 4);
   d |= static_cast<uint64_t>(mn_stride >> 4) << 16;
-  d |= static_cast<uint64_t>(256 >> 4) << 32;
+  d |= static_cast<uint64_t>(stride >> 4) << 32;
   d |= static_cast<uint64_t>(1) << 46;
   d |= static_cast<uint64_t>(6) << 61;  // layout type: SWIZZLE_32B
   return d;
