@@ -109,10 +109,11 @@ __device__ __forceinline__ long long block_prefix(long long v, long long* sums, 
 // product still forms 0 * v, which is NaN if v is infinite or NaN.  So the kernels take such values
 // out of the V tiles at positions that some row of the block does not see, remember per channel the
 // first position that holds +inf, -inf and NaN, and add them to the sums of the rows that do see them.
-__device__ __forceinline__ bool any_nonfinite(const uint4& v) {
-  auto hit = [&](uint32_t w) { return ((w & 0x7c00u) == 0x7c00u) || ((w & 0x7c000000u) == 0x7c000000u); };
-  return hit(v.x) || hit(v.y) || hit(v.z) || hit(v.w);
+__device__ __forceinline__ uint32_t nonfinite_bits(const uint4& v) {  // a full exponent carries into the sign's place
+  auto carry = [](uint32_t w) { return (w & 0x7c007c00u) + 0x04000400u; };
+  return (carry(v.x) | carry(v.y) | carry(v.z) | carry(v.w)) & 0x80008000u;
 }
+__device__ __forceinline__ bool any_nonfinite(const uint4& v) { return nonfinite_bits(v) != 0; }
 
 // Merges the splits of one row (one warp) and stores the fp16 row.  The records were written by
 // other SMs of the same launch: ld.global.cg.

@@ -138,8 +138,11 @@ __device__ __forceinline__ Line find_share(const Args& a, int shares, long long 
   const long long x = index * line.share;
   if (at <= x && x < at + mine) {
     for (int b = b0; b < b1; ++b) {
-      const Seq s = load_seq(a, b);
-      const long long len = a.num_kv_heads * blocks_length(a, s, s.blocks);
+      long long len = mine;
+      if (run > 1) {
+        const Seq s = load_seq(a, b);
+        len = a.num_kv_heads * blocks_length(a, s, s.blocks);
+      }
       if (x < at + len) {
         found->seq = b;
         found->at = at;
@@ -836,22 +839,6 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         // a block without keys (zeros) belongs to the stretch that it starts in
         if (u.tiles == 0 ? u.at < x0 : it.tile0 >= it.tile1) continue;
         it.part = it.tile0 == 0 && it.tile1 == u.tiles ? -1 : part_of(u, static_cast<int>(blockIdx.x), line.share);
-        if (it.tile0 == 0 && it.tile1 < u.tiles) {  // first part of a cut unit: list the parts for the merge
-          int n = 0;
-          for (int c = blockIdx.x; c * line.share < u.at + u.length; c += 32) {
-            const int part = (c + lane) * line.share < u.at + u.length ? part_of(u, c + lane, line.share) : -1;
-            const uint32_t has = __ballot_sync(0xffffffffu, part >= 0);
-            if (part >= 0) cut->parts[n + __popc(has & ((1u << lane) - 1u))] = part;
-            n += __popc(has);
-          }
-          if (lane == 0) {
-            cut->n = n;
-            cut->q_tok = it.q_tok;
-            cut->n_tok = it.n_tok;
-            cut->head = it.head;
-          }
-          listed = true;
-        }
         wait(&sm.item_empty[slot], slot_phase ^ 1u, 0);
         if (lane == 0) {
           sm.items[slot] = it;
@@ -894,6 +881,22 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           __syncwarp();
         }
         k_count += n;
+        if (it.tile0 == 0 && it.tile1 < u.tiles) {  // first part of a cut unit: list the parts for the merge
+          int n = 0;
+          for (int c = blockIdx.x; c * line.share < u.at + u.length; c += 32) {
+            const int part = (c + lane) * line.share < u.at + u.length ? part_of(u, c + lane, line.share) : -1;
+            const uint32_t has = __ballot_sync(0xffffffffu, part >= 0);
+            if (part >= 0) cut->parts[n + __popc(has & ((1u << lane) - 1u))] = part;
+            n += __popc(has);
+          }
+          if (lane == 0) {
+            cut->n = n;
+            cut->q_tok = it.q_tok;
+            cut->n_tok = it.n_tok;
+            cut->head = it.head;
+          }
+          listed = true;
+        }
       }
       if (cut != nullptr && !listed && lane == 0) cut->n = 0;
       if (!dead) {  // the end mark
@@ -960,29 +963,29 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           // rows that some row of the block does not see: no infinities, no NaN
           const int hid = min(max(it.pos0 + 1 - t0, 0), end);
           if (hid < kKeys) {
-            constexpr int kChunks = D / 8, kAhead = 4;  // loads under way per lane
-            for (int k0 = hid * kChunks + lane; k0 < kKeys * kChunks; k0 += 32 * kAhead) {
+            // A lane looks after one 16-byte column.  One test per eight chunks: one by one, a tile took 6000 clocks,
+            // and blocks of short contexts, nearly all of whose tiles are looked over, waited for it.
+            constexpr int kChunks = D / 8, kStep = 32 / kChunks, kAhead = 8;  // loads under way per lane
+            const int c = lane % kChunks, mine = lane / kChunks;
+            auto at = [&](int r) { return reinterpret_cast<uint4*>(tile + Sh::chunk(r, c)); };
+            for (int r0 = hid + mine; r0 < end; r0 += kStep * kAhead) {
               uint4 v[kAhead];
+              uint32_t hit = 0;
 #pragma unroll
-              for (int u = 0; u < kAhead; ++u) {
-                const int k = min(k0 + 32 * u, kKeys * kChunks - 1);
-                const int r = k / kChunks, c = k - r * kChunks;
-                v[u] = *reinterpret_cast<const uint4*>(tile + Sh::chunk(r, c));
-              }
+              for (int u = 0; u < kAhead; ++u) v[u] = *at(min(r0 + u * kStep, end - 1));
 #pragma unroll
-              for (int u = 0; u < kAhead; ++u) {
-                const int k = k0 + 32 * u;
-                if (k >= kKeys * kChunks) break;
-                const int r = k / kChunks, c = k - r * kChunks;
-                uint4* p = reinterpret_cast<uint4*>(tile + Sh::chunk(r, c));
-                if (r >= end) {
-                  *p = make_uint4(0, 0, 0, 0);
-                } else if (any_nonfinite(v[u])) {
-                  guard_take(v[u], static_cast<uint32_t>(t0 + r - (it.pos0 + 1)), special + c * 8, &sm.special_flag[slot]);
-                  *p = v[u];
+              for (int u = 0; u < kAhead; ++u) hit |= nonfinite_bits(v[u]);
+              if (hit != 0) {
+#pragma unroll 1
+                for (int r = r0; r < min(r0 + kStep * kAhead, end); r += kStep) {
+                  uint4 w = *at(r);
+                  if (!any_nonfinite(w)) continue;
+                  guard_take(w, static_cast<uint32_t>(t0 + r - (it.pos0 + 1)), special + c * 8, &sm.special_flag[slot]);
+                  *at(r) = w;
                 }
               }
             }
+            for (int r = end + mine; r < kKeys; r += kStep) *at(r) = make_uint4(0, 0, 0, 0);
             ptx::fence_proxy_async();
           }
           __syncwarp();
