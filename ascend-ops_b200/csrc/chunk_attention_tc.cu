@@ -2,8 +2,8 @@
 // head_dim 64 or 128, caches of either layout with P a multiple of 8, up to 128 query heads per kv head.
 //
 // One persistent CTA per SM takes an equal share of the batch's work (below) and computes two 128-row
-// score tiles at a time:  S_t = Q_t K^T and O_t += P_t V, t = 0, 1, both accumulators in TMEM (2 x 128 columns for
-// S, 2 x D for O; P_t is written back over S_t as fp16 and read from TMEM as the second product's left
+// score tiles at a time:  S_t = Q_t K^T and O_t += P_t V, t = 0, 1, both accumulators in TMEM (2 x 2 buffers of 64
+// columns for S, 2 x D for O; P_t is written back over S_t as fp16 and read from TMEM as the second product's left
 // operand).  While the tensor core works on one tile, a warpgroup takes the exponentials of the
 // other.  The two tiles are
 //   - the two halves of a block of more than 128 rows: both read the same K and V tile; or
@@ -13,8 +13,8 @@
 // issue the MMAs of tile 0 and 1, warp 10 goes through the CTA's work and announces every pair of kv tiles, warp 11
 // guards the V tiles (below), warps 12-15 walk the block table and issue the TMA loads.
 //
-// Online softmax: a row's reference maximum is only raised when the new maximum exceeds it by more
-// than 2^8 in the exponential, so the accumulator in TMEM is rescaled a few times per item instead of
+// Online softmax: a row's reference maximum is only raised when the new maximum would make a
+// probability larger than 2^8, so the accumulator in TMEM is rescaled a few times per item instead of
 // once per tile; probabilities are then up to 256, well inside fp16, and the final division
 // by the sum in fp32 makes up for any reference.
 //
@@ -97,7 +97,7 @@ struct Unit {
 __device__ __forceinline__ void set_block(const Args& a, Unit& u) {
   u.n_tok = min(a.block_tokens, u.s.n - u.block * a.block_tokens);
   u.pos0 = u.s.len - u.s.n + u.block * a.block_tokens;
-  u.tiles = (max(u.pos0 + u.n_tok, 0) + a.kv_tile - 1) / a.kv_tile;
+  u.tiles = (max(u.pos0 + u.n_tok, 0) + kKeys - 1) / kKeys;
   u.length = unit_length(a, u.s, u.block);
 }
 
@@ -489,6 +489,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 
   if (warp < static_cast<int>(kSoftmaxWarps)) {
     // =============================== softmax ===============================
+    // 256 threads x 176 + 256 x 80 = the launch's 512 x 128 registers
     asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     const int t = warp >> 2;                    // score tile
     const int row = (warp & 3) * 32 + lane;     // row of the tile = TMEM lane

@@ -407,3 +407,33 @@ def test_workspace_aligned_to_16_bytes_only(cabi):
             check(out, s)
             assert bool((raw[:at] == 0x5C).all()) and bool((raw[at + need:] == 0x5C).all())
             raw.fill_(0x5C)
+
+
+@pytest.mark.parametrize("hq,hkv,d,page,layout", [
+    (28, 4, 128, 64, NHD), (8, 2, 64, 16, NHD), (8, 2, 128, 16, NZ), (3, 3, 64, 8, NZ), (4, 2, 32, 3, NHD)])
+def test_many_non_finite_values(ops, hq, hkv, d, page, layout):
+    """Infinities and NaN in a tenth of a percent to a half of the values of the chunk and in a few before it: a row is
+    what those at its positions make it, channel by channel, and keeps its bits where there are none."""
+    n, L = 150, 410
+    s = make([(n, L), (20, 20)], hq, hkv, d, page, layout, seed=40)
+    clean = call(ops, s)
+    g = torch.Generator().manual_seed(41)
+    density = torch.zeros(L, 1, 1)
+    density[L - n:L - n + 40] = 0.001
+    density[L - n + 60:L - n + 70] = 0.02
+    density[L - 40:] = 0.5
+    density[5] = 0.01
+    put = torch.rand(L, hkv, d, generator=g) < density
+    bad = torch.tensor([float("inf"), float("-inf"), float("nan")])[torch.randint(0, 3, (L, hkv, d), generator=g)]
+    vc = s["vc"].cpu() if layout == NHD else s["vc"].cpu().transpose(1, 2).reshape(-1, page, hkv, d)
+    for p in range(L):
+        at = (int(s["table"][0, p // page]), p % page)
+        vc[at] = torch.where(put[p], bad[p].half(), vc[at])
+    s["vc"] = (vc if layout == NHD else vc.reshape(-1, page, hkv * d // 16, 16).transpose(1, 2)).contiguous().to(DEV)
+    got = call(ops, s).cpu()
+    assert torch.equal(got[n:], clean[n:].cpu())
+    seen = torch.where(put, bad, torch.zeros(())).double().cumsum(0)[L - n:]  # inf - inf and NaN: NaN
+    seen = seen.repeat_interleave(hq // hkv, 1)
+    hit = put.cumsum(0)[L - n:].repeat_interleave(hq // hkv, 1) > 0
+    assert torch.equal(got[:n][~hit], clean[:n].cpu()[~hit])
+    assert torch.equal(got[:n][hit].double().nan_to_num(nan=1.0), seen[hit].nan_to_num(nan=1.0))
