@@ -24,9 +24,10 @@ struct TensorTable {
   char* base[kMaxTensors];
 };
 
-// Copies `n` vectors, kUnroll in flight per thread.
+// Copies `n` vectors, kUnroll in flight per thread.  (No __restrict__ on inputs in this file: it would let them be
+// read as constants, but the kernels may be resident while the launch that writes them still runs.)
 template <typename V>
-__device__ __forceinline__ void copy_slice(const V* __restrict__ src, V* __restrict__ dst, int n) {
+__device__ __forceinline__ void copy_slice(const V* src, V* dst, int n) {
   for (int i0 = threadIdx.x; i0 < n; i0 += kCopyThreads * kUnroll) {
     V v[kUnroll];
 #pragma unroll
@@ -68,7 +69,7 @@ __device__ __forceinline__ void copy_disjoint(const TensorTable& tt, int tensors
 // columns of the page, which keeps the order without any exchange between threads.
 template <typename V>
 __global__ void __launch_bounds__(kCopyThreads)
-copy_pages_kernel(const TensorTable tt, int tensors, const int32_t* __restrict__ src, const int32_t* __restrict__ dst,
+copy_pages_kernel(const TensorTable tt, int tensors, const int32_t* src, const int32_t* dst,
                   int pairs, int num_pages, long long page_vecs, int hash_mask) {
   extern __shared__ int table[];  // hash_mask + 1 destinations, -1 = free
   __shared__ int conflict;
@@ -124,7 +125,7 @@ constexpr int kPlanThreads = 1024;
 constexpr int kMaxCompactPages = 1 << 19;  // bitmap and prefix counts in shared memory: 128 KB
 
 __global__ void __launch_bounds__(kPlanThreads)
-compact_plan_kernel(const int32_t* __restrict__ tables, const int32_t* __restrict__ page_counts, long long seqs, int width,
+compact_plan_kernel(const int32_t* tables, const int32_t* page_counts, long long seqs, int width,
                     int num_pages, int32_t* __restrict__ page_map, int32_t* __restrict__ num_live,
                     int32_t* __restrict__ moves, int32_t* __restrict__ move_src, int32_t* __restrict__ move_dst) {
   extern __shared__ uint32_t sm[];
@@ -138,13 +139,17 @@ compact_plan_kernel(const int32_t* __restrict__ tables, const int32_t* __restric
   for (int i = tid; i < words; i += kPlanThreads) bits[i] = 0;
   __syncthreads();
   pdl_wait();
-  const long long entries = seqs * width;
-  for (long long i = tid; i < entries; i += kPlanThreads) {
-    const long long b = i / width;
-    if (i - b * width < page_counts[b]) {
-      const int p = tables[i];
-      if (p >= 0 && p < num_pages) atomicOr(&bits[p >> 5], 1u << (p & 31));
+  const int entries = static_cast<int>(seqs * width);  // at most 2^26
+  for (int i0 = tid; i0 < entries; i0 += kPlanThreads * kUnroll) {
+    int page[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int i = i0 + u * kPlanThreads, b = i / width;
+      page[u] = i < entries && i - b * width < page_counts[b] ? tables[i] : -1;
     }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (page[u] >= 0 && page[u] < num_pages) atomicOr(&bits[page[u] >> 5], 1u << (page[u] & 31));
   }
   __syncthreads();
   // exclusive prefix of the words' live counts: a run of words per thread, then over the threads

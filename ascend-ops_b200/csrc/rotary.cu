@@ -91,14 +91,25 @@ struct RotArgs {
   bool interleaved;
 };
 
+// Plain (coherent) loads: the kernel may be resident while the launch that writes its inputs still runs, so they
+// are not constant for its whole life, as the non-coherent path wants.
+__device__ __forceinline__ uint4 load_piece(const __half* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+
 // Four neighbouring table entries, 8- (fp16) or 16-byte aligned.
 __device__ __forceinline__ void table4(const __half* t, float* v) {
-  const uint2 u = __ldg(reinterpret_cast<const uint2*>(t));
+  const uint2 u = *reinterpret_cast<const uint2*>(t);
   const float2 x = h2_to_f2(u.x), y = h2_to_f2(u.y);
   v[0] = x.x, v[1] = x.y, v[2] = y.x, v[3] = y.y;
 }
 __device__ __forceinline__ void table4(const float* t, float* v) {
-  const float4 u = __ldg(reinterpret_cast<const float4*>(t));
+  const float4 u = *reinterpret_cast<const float4*>(t);
   v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
 }
 
@@ -179,8 +190,8 @@ __global__ void __launch_bounds__(kRotThreads) rotary_vector_kernel(const RotArg
     if (head < heads) {
       const __half* in = head < a.num_heads ? a.q + t * a.q_stride + static_cast<long long>(head) * a.head_dim
                                             : a.k + t * a.k_stride + static_cast<long long>(head - a.num_heads) * a.head_dim;
-      v[n][0] = ld_stream(in + d0);
-      if (second) v[n][1] = ld_stream(in + d1);
+      v[n][0] = load_piece(in + d0);
+      if (second) v[n][1] = load_piece(in + d1);
     }
   }
   const int pos = a.position_ids[t];

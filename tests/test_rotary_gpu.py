@@ -169,3 +169,20 @@ def test_rotary_on_a_side_stream_and_in_a_graph(ops):
     assert torch.equal(cos, cos2) and torch.equal(sin, sin2)
     check_rotary(q, oq, pos, cos, sin, False)
     check_rotary(k, ok, pos, cos, sin, False)
+
+
+def test_tables_rewritten_between_calls(ops, cabi):
+    """Tables and inputs rewritten in place between two rotary calls of one stream, launch after launch without a
+    pause: every call sees what its predecessor wrote."""
+    f = [cabi.rotary_frequencies(128, base=b)[0] for b in (1e4, 3e5)]
+    q, k = torch.randn(700, 28, 128, device=DEV).half(), torch.randn(700, 4, 128, device=DEV).half()
+    pos = torch.randint(0, 700, (700,), device=DEV, dtype=torch.int32)
+    cos, sin = torch.empty(700, 64, device=DEV), torch.empty(700, 64, device=DEV)
+    outs = []
+    for i in range(12):
+        cabi.rotary_tables(f[i % 2], 1.0, 0, cos, sin, 1)
+        outs.append(ops.rotary(q, k, pos, cos, sin))
+    for i, (oq, ok) in enumerate(outs):
+        c, s = ops.rotary_tables(torch.tensor(f[i % 2], dtype=torch.float64), 700, dtype=torch.float32)
+        check_rotary(q, oq, pos, c, s, False)
+        check_rotary(k, ok, pos, c, s, False)
