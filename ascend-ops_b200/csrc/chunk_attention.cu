@@ -3,9 +3,12 @@
 //
 //   out[t] = sum_s softmax_s(q[t] . k[s] / sqrt(D)) v[s],  s = 0 .. position(t),
 // the softmax in one pass with running maximum and sum (fp32), base 2 with log2(e) folded into the
-// scale.  Probabilities are rounded to fp16 for the second product (at most 2^-11 of each, half a step,
-// like the rounding of the output itself, and of both signs, so the sum moves by less); the sums they are divided by
-// use the unrounded values.
+// scale.  Probabilities are rounded to fp16 for the second product, the type it multiplies; the sums they are divided by
+// use the unrounded values.  The rounding moves each by at most 2^-11 of itself (half a step, like the rounding of the
+// output itself, and of both signs, so the sum moves by less) as long as it is above 2^-14; a smaller one moves by up to
+// 2^-25, and below 2^-25 it is lost, always in one direction.  So the exponents are lifted by 15 here (by 7 in the
+// tcgen05 kernel, whose reference may be 2^8 below the maximum): the largest is 2^15, still fp16, and what rounding
+// takes from a small one is at most 2^-40 (2^-32) of the largest.  The sums carry the same factor.
 //
 // Lengths are device data, so the work is planned on the device: a one-CTA launch cuts the batch
 // into items (blocks of tokens x heads x ranges of kv tiles), longest ranges of a sequence first,
@@ -144,6 +147,7 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_attention_plan_kernel(Args
 // ---- general kernel ---------------------------------------------------------------------------
 constexpr int kThreads = 128;
 constexpr int kRows = 64;
+constexpr float kLift = 15.f;  // a row's largest probability is 2^15: the small ones stay away from fp16's subnormals
 
 template <int D>
 struct GeneralShape {
@@ -314,6 +318,7 @@ __global__ void __launch_bounds__(kThreads) chunk_attention_general_kernel(Args 
       const float n_lo = fmaxf(m_lo, mx_lo), n_hi = fmaxf(m_hi, mx_hi);
       const float u_lo = n_lo == -INFINITY ? 0.f : n_lo, u_hi = n_hi == -INFINITY ? 0.f : n_hi;
       const float f_lo = exp2f(m_lo - u_lo), f_hi = exp2f(m_hi - u_hi);
+      const float z_lo = u_lo - kLift, z_hi = u_hi - kLift;
       m_lo = n_lo;
       m_hi = n_hi;
       l_lo *= f_lo;
@@ -330,8 +335,8 @@ __global__ void __launch_bounds__(kThreads) chunk_attention_general_kernel(Args 
         uint32_t pf[4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float p0 = exp2f(s[2 * kb + h][0] - u_lo), p1 = exp2f(s[2 * kb + h][1] - u_lo);
-          const float p2 = exp2f(s[2 * kb + h][2] - u_hi), p3 = exp2f(s[2 * kb + h][3] - u_hi);
+          const float p0 = exp2f(s[2 * kb + h][0] - z_lo), p1 = exp2f(s[2 * kb + h][1] - z_lo);
+          const float p2 = exp2f(s[2 * kb + h][2] - z_hi), p3 = exp2f(s[2 * kb + h][3] - z_hi);
           l_lo += p0 + p1;
           l_hi += p2 + p3;
           pf[2 * h] = f2_to_h2(p0, p1);

@@ -14,9 +14,9 @@
 // guards the V tiles (below), warps 12-15 walk the block table and issue the TMA loads.
 //
 // Online softmax: a row's reference maximum is only raised when the new maximum would make a
-// probability larger than 2^8, so the accumulator in TMEM is rescaled a few times per item instead of
-// once per tile; probabilities are then up to 256, well inside fp16, and the final division
-// by the sum in fp32 makes up for any reference.
+// probability larger than 2^8 times that of the reference, so the accumulator in TMEM is rescaled a few times per item
+// instead of once per tile.  The reference's own probability is taken as 2^7: the largest is then 2^15, still inside fp16,
+// the small ones stay away from its subnormals, and the final division by the sum in fp32 makes up for any factor.
 //
 // Bounds.  With more than one score tile per block, the tensor core (a pair of tiles of 128 rows x 64 keys, D = 128: 1280
 // clocks) and the special-function unit (1024) are near each other, and what is lost is the way between them: 4096
@@ -48,6 +48,7 @@ constexpr int kKeys = 64;   // keys of a kv tile
 constexpr int kMaskRing = 16;
 constexpr int kMmaWarp = 8, kPlanWarp = 10, kGuardWarp = 11, kLoadWarp = 12;  // MMA: 8 and 9, one per score tile
 constexpr uint32_t kSoftmaxWarps = 8;
+constexpr float kLift = 7.f, kWindow = 8.f;  // log2 of the reference's probability, and of what the largest is over it
 constexpr int kErrBase = 21;  // 21 loads, 22 MMA, 23 softmax, 24 guard, 25 misaligned shared memory
 
 __device__ int g_ca_status = 0;
@@ -557,7 +558,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         const uint64_t scale2 = pair(scale, scale);
         uint64_t sum2[2];
         auto exponentials = [&](int from, int to) {
-          const float shift = m == -INFINITY ? 0.f : -m * scale;
+          const float shift = m == -INFINITY ? 0.f : kLift - m * scale;
           const uint64_t shift2 = pair(shift, shift);
           if (from == 0) sum2[0] = sum2[1] = 0;
 #pragma unroll
@@ -593,7 +594,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           } else if (raise) {
             f = ex2((m - top) * scale);  // from -inf: 0
             m = top;
-            limit = top + 8.f / scale;
+            limit = top + kWindow / scale;
             l *= f;
           }
           if (i > 0) {

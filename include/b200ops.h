@@ -452,6 +452,8 @@ int b200ops_rotary(const void* q, const void* k, const int32_t* position_ids, co
  * not written.  query_starts must not decrease (rows outside [0, num_tokens) are left out).
  * What lies in the cache behind a token's position -- unused slots, other tokens of the chunk -- has no
  * influence on its row, also if it is infinite or NaN.
+ * Scores, probabilities and sums are f32; for the product with V the probabilities are rounded to f16, which moves each by
+ * at most 2^-11 of itself, or 2^-32 of the row's largest.
  * head_dim in {32, 64, 128, 256}; num_tokens <= 2^24.  Lengths are read on the device only, so a captured
  * graph serves any lengths of its shape.  Results do not depend on scheduling (bitwise repeatable).
  */
