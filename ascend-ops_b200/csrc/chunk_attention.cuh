@@ -116,7 +116,8 @@ __device__ __forceinline__ uint32_t nonfinite_bits(const uint4& v) {  // a full 
 __device__ __forceinline__ bool any_nonfinite(const uint4& v) { return nonfinite_bits(v) != 0; }
 
 // Merges the splits of one row (one warp) and stores the fp16 row.  The records were written by
-// other SMs of the same launch: ld.global.cg.
+// other SMs of the same launch: ld.global.cg.  A part whose weight underflows is added like any other: if it
+// holds an infinity or a NaN, the result must not be finite.
 __device__ __forceinline__ void merge_row(const Args& a, int row0, int rows, int r, int n_splits, __half* out, int lane) {
   const float2* ml = a.part_ml + row0 + r;
   float m = -INFINITY;
@@ -139,10 +140,7 @@ __device__ __forceinline__ void merge_row(const Args& a, int row0, int rows, int
     const float* o = a.part_o + (static_cast<size_t>(row0) + static_cast<size_t>(s) * rows + r) * a.head_dim;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < per) {
-        const float v = __ldcg(o + lane + 32 * i);
-        if (w != 0.f) acc[i] = fmaf(w, v, acc[i]);
-      }
+      if (i < per) acc[i] = fmaf(w, __ldcg(o + lane + 32 * i), acc[i]);
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i)

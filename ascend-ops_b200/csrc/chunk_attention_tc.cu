@@ -1070,7 +1070,7 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_attention_merge_kernel(co
           const float4 x = *reinterpret_cast<const float4*>(a.part_o + (pr + r) * D + k * 32 + channel);
           const float v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[j][4 * k + e] = fmaf(w, w != 0.f ? v[e] : 0.f, acc[j][4 * k + e]);
+          for (int e = 0; e < 4; ++e) acc[j][4 * k + e] = fmaf(w, v[e], acc[j][4 * k + e]);  // 0 * inf: see merge_row
         }
       }
     }

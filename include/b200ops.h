@@ -452,6 +452,8 @@ int b200ops_rotary(const void* q, const void* k, const int32_t* position_ids, co
  * not written.  query_starts must not decrease (rows outside [0, num_tokens) are left out).
  * What lies in the cache behind a token's position -- unused slots, other tokens of the chunk -- has no
  * influence on its row, also if it is infinite or NaN.
+ * An infinite or NaN value at a position that a row sees makes its channel of the row infinite or NaN: by the formula
+ * where the position's probability is above 2^-31 of the row's largest, either of the two where it is smaller.
  * Scores, probabilities and sums are f32; for the product with V the probabilities are rounded to f16, which moves each by
  * at most 2^-11 of itself, or 2^-32 of the row's largest.
  * head_dim in {32, 64, 128, 256}; num_tokens <= 2^24.  Lengths are read on the device only, so a captured

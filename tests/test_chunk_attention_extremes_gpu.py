@@ -1,4 +1,5 @@
-"""ops.chunked_paged_attention where probabilities are tiny: what many of them add up to.
+"""ops.chunked_paged_attention where probabilities are tiny: what many of them add up to, and what a non-finite value of
+such a key does.
 
 The scores are set through channel 0 alone: q has sqrt(D) there and 0 elsewhere, so a key's score is its value in
 channel 0, up to the rounding of sqrt(D) to float16, which the reference applies too.
@@ -82,3 +83,23 @@ def test_many_small_probabilities(ops, hq, hkv, d, page, layout, news):
             err = (out[t + i] - want).abs()
             assert bool((err <= tol).all()), (n, i, float((err / tol).max()), float(want.mean()))
         t += n
+
+
+@pytest.mark.parametrize("hq,hkv,d,page,layout", SHAPES)
+@pytest.mark.parametrize("length", [300, 9000])  # in one piece, and cut into parts
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_non_finite_values_of_unlikely_keys(ops, hq, hkv, d, page, layout, length, value):
+    """A visible key 300 below the highest score, which is the last one: its probability is 0 in fp32, but by the definition
+    it is not, so a non-finite value of it makes its channel non-finite; the other channels stay as they were."""
+    g = torch.Generator().manual_seed(length)
+    scores = torch.randn(length, generator=g) - 300
+    scores[-1] = 0
+    values = torch.randn(length, hkv, d, generator=g)
+    clean = call(ops, state([1, 1], scores, values, hq, hkv, page, layout))
+    assert bool(clean.isfinite().all())
+    values[17, 0, 5] = value
+    got = call(ops, state([1, 1], scores, values, hq, hkv, page, layout))
+    hit = torch.zeros(hq, d, dtype=torch.bool, device=DEV)
+    hit[:hq // hkv, 5] = True
+    assert not bool(got[:, hit].isfinite().any())
+    assert torch.equal(got[:, ~hit], clean[:, ~hit])
