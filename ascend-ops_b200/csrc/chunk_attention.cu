@@ -251,6 +251,7 @@ __global__ void __launch_bounds__(kThreads) chunk_attention_general_kernel(Args 
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m_lo = -INFINITY, m_hi = -INFINITY, l_lo = 0.f, l_hi = 0.f;
+    bool seen_lo = false, seen_hi = false;  // the row sees a key
     const int kv_len = it.pos0 + it.n_tok;
     const int32_t* table = a.block_tables + static_cast<size_t>(it.seq) * a.max_pages_per_seq;
 
@@ -300,6 +301,9 @@ __global__ void __launch_bounds__(kThreads) chunk_attention_general_kernel(Args 
       }
       const uint64_t mask = s_mask[0] | (static_cast<uint64_t>(s_mask[1]) << 32);
       const int lim_lo = pos_lo - t0, lim_hi = pos_hi - t0;  // last visible column
+      auto visible = [&](int lim) { return lim < 0 ? 0 : mask & (lim >= 63 ? ~0ull : (2ull << lim) - 1); };
+      seen_lo |= visible(lim_lo) != 0;
+      seen_hi |= visible(lim_hi) != 0;
       float mx_lo = -INFINITY, mx_hi = -INFINITY;
 #pragma unroll
       for (int nb = 0; nb < kTile / 8; ++nb)
@@ -365,8 +369,10 @@ __global__ void __launch_bounds__(kThreads) chunk_attention_general_kernel(Args 
         for (int j = 0; j < 4; ++j)
           o[i][j] += special_term(special, D, i * 8 + 2 * t4 + (j & 1), j < 2 ? pos_lo : pos_hi);
     }
+    if (seen_lo) m_lo = fmaxf(m_lo, kLowest);
+    if (seen_hi) m_hi = fmaxf(m_hi, kLowest);
     if (it.n_splits == 1) {
-      const float i_lo = l_lo == 0.f ? 0.f : 1.0f / l_lo, i_hi = l_hi == 0.f ? 0.f : 1.0f / l_hi;
+      const float i_lo = row_factor(m_lo, l_lo), i_hi = row_factor(m_hi, l_hi);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int r = half ? r_hi : r_lo;

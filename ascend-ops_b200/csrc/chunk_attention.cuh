@@ -115,6 +115,13 @@ __device__ __forceinline__ uint32_t nonfinite_bits(const uint4& v) {  // a full 
 }
 __device__ __forceinline__ bool any_nonfinite(const uint4& v) { return nonfinite_bits(v) != 0; }
 
+// Maximum of a row that sees keys, but none with a score above -inf: its softmax is 0 / 0.  Below any score that finite
+// operands can have, so a part with such a key decides; -inf stays the maximum of a row that sees no key.
+constexpr float kLowest = -1e38f;
+
+// What a row's sums are multiplied with: sum 0 and nothing seen: zeros; a NaN sum stays NaN.
+__device__ __forceinline__ float row_factor(float m, float l) { return l == 0.f ? (m == -INFINITY ? 0.f : NAN) : 1.0f / l; }
+
 // Merges the splits of one row (one warp) and stores the fp16 row.  The records were written by
 // other SMs of the same launch: ld.global.cg.  A part whose weight underflows is added like any other: if it
 // holds an infinity or a NaN, the result must not be finite.
@@ -130,7 +137,7 @@ __device__ __forceinline__ void merge_row(const Args& a, int row0, int rows, int
     l += v.y * exp2f(v.x - m_use);
   }
   l = warp_sum(l);
-  const float inv = l == 0.f ? 0.f : 1.0f / l;  // nothing visible: zeros; a NaN sum stays NaN
+  const float inv = row_factor(m, l);
   const int per = a.head_dim >> 5;  // channels lane, lane + 32, ...
   float acc[8];
 #pragma unroll

@@ -528,6 +528,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       const int steps = dual ? n : (n + 1 - t) / 2;  // kv tiles of this warpgroup
       float m = -INFINITY, l = 0.f;  // reference maximum (raw scores) and sum
       float limit = -INFINITY;       // scores up to here keep the reference
+      uint32_t seen = 0;             // the row sees a key
       const int row_pos = pos - it.tile0 * kKeys;                 // this row's position behind the first key
       const int warp_pos = __shfl_sync(0xffffffffu, row_pos, 0);  // the least of the warp's
       int off = dual ? 0 : t * kKeys;                             // first key of the tile
@@ -551,7 +552,10 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 #pragma unroll
             for (int c = 0; c < 32; ++c)
               if (!((bits >> c) & 1u)) s[g][c] = __float_as_uint(-INFINITY);
+            seen |= bits;
           }
+        } else {
+          seen = 1;
         }
         off += dual ? kKeys : 2 * kKeys;
         uint32_t p[32];
@@ -652,6 +656,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 #pragma unroll 1
         for (int i = 0; i < steps; ++i) step(i, s);
       }
+      if (seen) m = fmaxf(m, kLowest);
       if (steps > 1) pv_phase ^= 1u;
       k_count += n;
 
@@ -717,7 +722,7 @@ chunk_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         }
       };
       const size_t record = static_cast<size_t>(it.part) * slot_rows + my_tok * group + head;
-      const float inv = l == 0.f ? 0.f : 1.0f / l;  // nothing visible: zeros; a NaN sum stays NaN
+      const float inv = row_factor(m, l);
 #pragma unroll 1
       for (int c = c0; c < c1; c += 32) {
         float v[32];
@@ -1038,7 +1043,7 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_attention_merge_kernel(co
   const int step = gridDim.y * (kMergeThreads / 32) * warp_rows;
   for (int r_warp = (blockIdx.y * (kMergeThreads / 32) + warp) * warp_rows; r_warp < rows; r_warp += step) {
     const int r0 = r_warp + row;
-    float m[kMergeRows], l[kMergeRows], acc[kMergeRows][kPer * 4];
+    float m[kMergeRows], top[kMergeRows], l[kMergeRows], acc[kMergeRows][kPer * 4];
 #pragma unroll
     for (int j = 0; j < kMergeRows; ++j) {
       m[j] = -INFINITY;
@@ -1055,6 +1060,7 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_attention_merge_kernel(co
     for (int j = 0; j < kMergeRows; ++j) {
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) m[j] = fmaxf(m[j], __shfl_xor_sync(0xffffffffu, m[j], o));
+      top[j] = m[j];
       if (m[j] == -INFINITY) m[j] = 0.f;
     }
     for (int i = sub; i < n; i += parts) {
@@ -1085,7 +1091,7 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_attention_merge_kernel(co
       }
       const int r = r0 + j;
       if (r >= rows) continue;
-      const float inv = l[j] == 0.f ? 0.f : 1.0f / l[j];  // nothing visible: zeros; a NaN sum stays NaN
+      const float inv = row_factor(top[j], l[j]);
       const int tok = r / a.group;
       __half* dst = a.out + (static_cast<size_t>(cut.q_tok + tok) * a.num_heads + cut.head * a.group + r - tok * a.group) * D + channel;
 #pragma unroll

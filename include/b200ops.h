@@ -447,7 +447,7 @@ int b200ops_rotary(const void* q, const void* k, const int32_t* position_ids, co
  *   block_tables : int32 [bs, max_pages_per_seq]; caches in `layout`, num_pages pages of page_size tokens.
  * Token i of a sequence with n new tokens and L in context stands at position p = L - n + i and
  *   out = softmax(q . K[0..p]^T / sqrt(head_dim)) . V[0..p]   (query heads share kv heads as in paged_attention)
- * A token with p < 0 gets zeros.  A block-table entry outside [0, num_pages) leaves its page's tokens out.
+ * A token with p < 0 gets zeros; one whose visible scores are all -inf gets NaN (0 / 0).  A block-table entry outside [0, num_pages) leaves its page's tokens out.
  * A context above max_pages_per_seq * page_size is taken as that.  Rows that belong to no sequence are
  * not written.  query_starts must not decrease (rows outside [0, num_tokens) are left out).
  * What lies in the cache behind a token's position -- unused slots, other tokens of the chunk -- has no

@@ -1,5 +1,5 @@
 """ops.chunked_paged_attention where probabilities are tiny: what many of them add up to, and what a non-finite value of
-such a key does.
+such a key does; and scores of -inf.
 
 The scores are set through channel 0 alone: q has sqrt(D) there and 0 elsewhere, so a key's score is its value in
 channel 0, up to the rounding of sqrt(D) to float16, which the reference applies too.
@@ -103,3 +103,37 @@ def test_non_finite_values_of_unlikely_keys(ops, hq, hkv, d, page, layout, lengt
     hit[:hq // hkv, 5] = True
     assert not bool(got[:, hit].isfinite().any())
     assert torch.equal(got[:, ~hit], clean[:, ~hit])
+
+
+@pytest.mark.parametrize("hq,hkv,d,page,layout", SHAPES)
+@pytest.mark.parametrize("low,length,new", [(6, 12, 12), (300, 300, 40), (200, 300, 150), (300, 700, 700), (9000, 9000, 1),
+                                            (8999, 9000, 3), (8900, 9000, 200), (4000, 9000, 1)])
+def test_scores_of_minus_infinity(ops, hq, hkv, d, page, layout, low, length, new):
+    """The first `low` keys have the score -inf.  A row that sees no other key is NaN (0 / 0); behind the first other key
+    those have no weight."""
+    g = torch.Generator().manual_seed(low)
+    scores = torch.zeros(length)
+    scores[:low] = float("-inf")
+    values = torch.randn(length, hkv, d, generator=g)
+    got = call(ops, state([new, new], scores, values, hq, hkv, page, layout))
+    nothing = max(0, low - (length - new))  # rows that see keys of -inf only
+    for t in (0, new):
+        assert bool(got[t:t + nothing].isnan().all())
+        if nothing < new:
+            first = max(low, length - new)  # position of the first row that sees another key
+            mean = values[low:].half().double().cumsum(0)[first - low:] / torch.arange(first - low + 1, length - low + 1)[:, None, None]
+            size = values[low:].half().double().abs().cumsum(0)[first - low:] / torch.arange(first - low + 1, length - low + 1)[:, None, None]
+            # equal weights: exact in float16; the sums' and the result's rounding are left
+            tol = 2.0 ** -11 * mean.abs() + 2.0 ** -25 + 2 * (length / 8 + 64) * 2.0 ** -23 * size
+            want, tol = (x.repeat_interleave(hq // hkv, 1).to(DEV) for x in (mean, tol))
+            assert bool(((got[t + nothing:t + new].double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("hq,hkv,d,page,layout", SHAPES)
+def test_rows_that_see_nothing_beside_scores_of_minus_infinity(ops, hq, hkv, d, page, layout):
+    """More new tokens than context: the first rows stand before every key and are zeros, the others see -inf only."""
+    s = state([20], torch.full((12,), float("-inf")), torch.randn(12, hkv, d), hq, hkv, page, layout)
+    got = call(ops, s)
+    assert bool((got[:8] == 0).all()) and bool(got[8:].isnan().all())
+    s["table"].fill_(-1)
+    assert bool((call(ops, s) == 0).all())
