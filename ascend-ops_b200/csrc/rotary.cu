@@ -21,11 +21,32 @@ namespace {
 
 constexpr int kMaxHalf = 256;
 constexpr double kTwoPi = 6.283185307179586476925286766559;
+constexpr double kTwoPiRest = 2.4492935982947064e-16;  // 2 pi - kTwoPi
 
-// Turns (periods) per position of every frequency, by value in the launch.
-struct TurnTable {
-  double turns[kMaxHalf];
+// Frequencies, by value in the launch.
+struct FrequencyTable {
+  double f[kMaxHalf];
 };
+
+// Turns (periods) per position, f / 2 pi, as the sum of two doubles: by itself the first is off by 2^-54 of itself, and so
+// is a position's angle, which at position 2^31 is more than the last bit of an fp32 table.
+struct Turns {
+  double high, low;
+};
+
+__device__ __forceinline__ Turns turns_of(double f) {
+  Turns t;
+  t.high = f / kTwoPi;
+  t.low = (fma(-t.high, kTwoPi, f) - t.high * kTwoPiRest) / kTwoPi;
+  return t;
+}
+
+// position * t less whole turns, in turns: the product's rounding error is kept (fma), so what is left are a few
+// roundings of numbers below one.
+__device__ __forceinline__ double reduced(double position, Turns t) {
+  const double p = position * t.high;
+  return (p - rint(p)) + fma(position, t.low, fma(position, t.high, -p));
+}
 
 __device__ __forceinline__ void store_pair(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_pair(__half* p, float v) { *p = __float2half_rn(v); }
@@ -33,19 +54,19 @@ __device__ __forceinline__ void store_pair(__half* p, float v) { *p = __float2ha
 constexpr int kTableThreads = 256;
 
 // One thread = one frequency over `rows` consecutive positions.  The angle of the first one is
-// reduced exactly enough in double (position * turns, minus the nearest whole number: the error is
-// 2^-53 of the number of turns, where fp32 would lose every digit past position 10^7); the others
-// follow by rotating (cos, sin) by one step's angle, four double operations per entry, whose error
-// grows by about 2^-53 per row and stays far below the table's last bit.
+// reduced to 2^-50 at any position (fp32 would lose every digit past position 10^7, a plain double product
+// one more with every doubling); the others follow by rotating (cos, sin) by one step's angle, four double operations per
+// entry.  A step adds an error of at most 2^-50, so all 64 stay below 2^-43 of the amplitude: 2^-18 of half a step of an
+// fp32 entry between 1/2 and 1.
 // Bound: writing the tables.  Neighbouring threads hold neighbouring frequencies of one row, so a
 // warp stores whole sectors: 262144 positions x 64 frequencies in fp32 (134 MB) take 26 us = 5.2 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(kTableThreads)
-rotary_tables_kernel(const TurnTable tt, T* __restrict__ cos_t, T* __restrict__ sin_t, long long start,
+rotary_tables_kernel(const FrequencyTable ft, T* __restrict__ cos_t, T* __restrict__ sin_t, long long start,
                      long long num_positions, int half, int rows, double amplitude) {
-  __shared__ double turns[kMaxHalf];
+  __shared__ Turns turns[kMaxHalf];
   pdl_trigger();
-  for (int i = threadIdx.x; i < half; i += kTableThreads) turns[i] = tt.turns[i];
+  for (int i = threadIdx.x; i < half; i += kTableThreads) turns[i] = turns_of(ft.f[i]);
   __syncthreads();
   pdl_wait();
   const long long item = static_cast<long long>(blockIdx.x) * kTableThreads + threadIdx.x;
@@ -54,11 +75,10 @@ rotary_tables_kernel(const TurnTable tt, T* __restrict__ cos_t, T* __restrict__ 
   const long long p0 = group * rows;
   if (p0 >= num_positions) return;
   const int n = static_cast<int>(min(static_cast<long long>(rows), num_positions - p0));
-  const double f = turns[j];
-  double angle = static_cast<double>(start + p0) * f;
+  const Turns t = turns[j];
   double c, s, cs, ss;
-  sincospi(2.0 * (angle - rint(angle)), &s, &c);
-  sincospi(2.0 * (f - rint(f)), &ss, &cs);
+  sincospi(2.0 * reduced(static_cast<double>(start + p0), t), &s, &c);
+  sincospi(2.0 * reduced(1.0, t), &ss, &cs);
   c *= amplitude;
   s *= amplitude;
   T* pc = cos_t + p0 * half + j;
@@ -341,11 +361,11 @@ extern "C" int b200ops_rotary_tables(const double* frequencies, int64_t half, do
                   "rotary_tables: unknown table type %d", table_type);
   B200OPS_REQUIRE(std::isfinite(amplitude), "rotary_tables: amplitude must be finite");
   B200OPS_REQUIRE(frequencies, "rotary_tables: null pointer");
-  TurnTable tt;
+  FrequencyTable ft;
   for (int64_t j = 0; j < half; ++j) {
     B200OPS_REQUIRE(std::isfinite(frequencies[j]) && std::fabs(frequencies[j]) <= 1e6,
                     "rotary_tables: frequency %lld is %g", (long long)j, frequencies[j]);
-    tt.turns[j] = frequencies[j] / kTwoPi;
+    ft.f[j] = frequencies[j];
   }
   if (num_positions == 0) return B200OPS_OK;
   B200OPS_REQUIRE(cos_table && sin_table, "rotary_tables: null pointer");
@@ -355,11 +375,11 @@ extern "C" int b200ops_rotary_tables(const double* frequencies, int64_t half, do
   const dim3 grid(static_cast<unsigned>((items + kTableThreads - 1) / kTableThreads));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (table_type == B200OPS_TABLE_F32)
-    B200OPS_CUDA(launch_kernel(rotary_tables_kernel<float>, grid, dim3(kTableThreads), 0, st, tt,
+    B200OPS_CUDA(launch_kernel(rotary_tables_kernel<float>, grid, dim3(kTableThreads), 0, st, ft,
                                static_cast<float*>(cos_table), static_cast<float*>(sin_table), (long long)start,
                                (long long)num_positions, (int)half, (int)rows, amplitude));
   else
-    B200OPS_CUDA(launch_kernel(rotary_tables_kernel<__half>, grid, dim3(kTableThreads), 0, st, tt,
+    B200OPS_CUDA(launch_kernel(rotary_tables_kernel<__half>, grid, dim3(kTableThreads), 0, st, ft,
                                static_cast<__half*>(cos_table), static_cast<__half*>(sin_table), (long long)start,
                                (long long)num_positions, (int)half, (int)rows, amplitude));
   return B200OPS_OK;

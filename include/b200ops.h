@@ -412,7 +412,8 @@ int b200ops_moe_combine(const void* returned, const int32_t* slot_to_row, const 
  *   *amplitude is 1 except for YARN.  frequencies: double [rotary_dim/2], host memory; rotary_dim <= 512.
  * rotary_tables: cos_table[p, j] = amplitude * cos((start + p) * frequencies[j]), sin_table likewise,
  *   [num_positions, half] f16 or f32 (table_type).  `frequencies` is read on the host before the
- *   call returns.  Angles are reduced in double: exact to the table's last bit at any position.
+ *   call returns.  An entry is the formula's value, off by at most 2^-43 of the amplitude, rounded once to its type,
+ *   at any position (frequencies up to 1e6).
  * rotary: q [num_tokens, num_heads, head_dim] and k [num_tokens, num_kv_heads, head_dim], f16, with
  *   q_stride / k_stride elements from one token to the next (views of a packed projection);
  *   out_q, out_k dense.  Tables [max_pos, rotary_dim/2] of table_type.  Pairs are (x[j], x[j + rotary_dim/2]),
