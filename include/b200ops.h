@@ -404,9 +404,9 @@ int b200ops_moe_combine(const void* returned, const int32_t* slot_to_row, const 
  *     NONE    f_j
  *     LINEAR  f_j / factor
  *     NTK     base * factor^(rotary_dim/(rotary_dim-2)) in place of base
- *     YARN    f_j / factor below index ceil(i(low)), f_j above floor(i(high)), linear in j between,
- *             i(n) = the index that turns n times over original_positions; *amplitude = 0.1 ln(factor) + 1
- *             (usual: low 1, high 32)
+ *     YARN    f_j up to index floor(i(high)), f_j / factor from index ceil(i(low)) on, linear in j between,
+ *             i(n) = the index that turns n times over original_positions (i(high) < i(low));
+ *             *amplitude = 0.1 ln(factor) + 1 (usual: low 1, high 32)
  *     BANDS   share ((original_positions f_j / 2 pi) - low) / (high - low), clamped to [0, 1], of f_j,
  *             the rest of f_j / factor (usual: low 1, high 4)
  *   *amplitude is 1 except for YARN.  frequencies: double [rotary_dim/2], host memory; rotary_dim <= 512.
