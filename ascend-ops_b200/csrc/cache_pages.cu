@@ -241,7 +241,8 @@ int vector_bytes(void* const* tensors, int64_t n, int64_t page_bytes) {
 int check_tensors(const char* op, void* const* tensors, int64_t n, int64_t num_pages, int64_t page_bytes) {
   B200OPS_REQUIRE(n >= 1 && n <= kMaxListed && tensors, "%s: one to %d cache tensors, got %lld", op, kMaxListed,
                   (long long)n);
-  B200OPS_REQUIRE(num_pages >= 1 && num_pages <= 0x7fffffffLL && page_bytes >= 1 && page_bytes <= (1LL << 40),
+  constexpr int64_t kMaxBytes = 1LL << 48;  // of a tensor: more than can be addressed, and the sums below cannot wrap
+  B200OPS_REQUIRE(num_pages >= 1 && num_pages <= 0x7fffffffLL && page_bytes >= 1 && page_bytes <= kMaxBytes / num_pages,
                   "%s: bad cache shape pages=%lld page_bytes=%lld", op, (long long)num_pages, (long long)page_bytes);
   // Two tensors that share memory would be written through both: refuse instead of racing.
   uintptr_t sorted[kMaxListed];
