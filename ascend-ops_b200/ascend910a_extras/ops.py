@@ -161,5 +161,6 @@ def compact_pages(
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Move the pages named by the first page_counts[b] entries of each row of block_tables to the
     front of every cache, in place.  Returns (new block tables, page_map [pages]: the new number of
-    each live page, -1 for the others, num_live [1])."""
+    each live page, -1 for the others, num_live [1]).  Every column is looked at: hand over the columns
+    in use of a wide table."""
     return _C.ops.compact_pages(list(caches), block_tables, page_counts)

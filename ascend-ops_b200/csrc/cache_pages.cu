@@ -66,7 +66,8 @@ __device__ __forceinline__ void copy_disjoint(const TensorTable& tt, int tensors
 // for itself with a hash set of the destinations in shared memory (about 1 us for 1000 pairs,
 // hidden by the first copies' latency; a planning launch of its own would cost more).  Independent
 // pairs are spread over the grid.  Otherwise every thread walks the whole list for its own 16-byte
-// columns of the page, which keeps the order without any exchange between threads.
+// columns of the page, which keeps the order without any exchange between threads, at one load and store
+// at a time: 600 pairs of 128 KB in 8 tensors take 205 us if they are independent and 408 us if a single pair is not.
 template <typename V>
 __global__ void __launch_bounds__(kCopyThreads)
 copy_pages_kernel(const TensorTable tt, int tensors, const int32_t* src, const int32_t* dst,
@@ -119,7 +120,10 @@ copy_pages_kernel(const TensorTable tt, int tensors, const int32_t* src, const i
   }
 }
 
-// compact_pages, first launch: one CTA finds the live pages and where each goes.
+// compact_pages, first launch: one CTA finds the live pages and where each goes.  Its time goes with the size of
+// the tables, used or not (an entry costs its row's count, then itself, from L2): 28 us for 256 rows of 128
+// entries, 130 us for 64 of 8192, 500 us for 256 of 8192, with 100 entries of each row in use (both launches, nothing to
+// move).  A caller with wide tables hands over the columns in use.
 // Workspace: move count, then the sources and the destinations of the moves.
 constexpr int kPlanThreads = 1024;
 constexpr int kMaxCompactPages = 1 << 19;  // bitmap and prefix counts in shared memory: 128 KB

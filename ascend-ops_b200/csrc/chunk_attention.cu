@@ -192,8 +192,9 @@ __device__ __forceinline__ float special_term(const int* special, int head_dim, 
 
 // Four warps, each 16 of the block's 64 rows; K and V tiles go through shared memory, the products
 // run on warp-level tensor-core instructions (fp16 in, fp32 out).  The path for shapes the tcgen05
-// kernel does not take (head_dim 32 or 256, pages that are not a multiple of 8 tokens); bound by the load latency of its
-// single-buffered tiles: 4096 new tokens at context 16384, 28 heads of 128, take 9.3 ms (0.09 PFLOP/s).
+// kernel does not take (head_dim 32 or 256, pages that are not a multiple of 8 tokens, more than 128 query heads per kv
+// head); bound by the load latency of its single-buffered tiles: 4096 new tokens at context 16384, 28 heads of 128, take
+// 9.3 ms (0.09 PFLOP/s); 2048 at context 8192, 16 heads of 256 on 4, 2.6 ms, 32 heads of 32 on 8, 0.74 ms (0.09, 0.08).
 template <int D>
 __global__ void __launch_bounds__(kThreads) chunk_attention_general_kernel(Args a) {
   using G = GeneralShape<D>;

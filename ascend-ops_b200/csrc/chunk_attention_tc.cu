@@ -18,14 +18,18 @@
 // instead of once per tile.  The reference's own probability is taken as 2^7: the largest is then 2^15, still inside fp16,
 // the small ones stay away from its subnormals, and the final division by the sum in fp32 makes up for any factor.
 //
-// Bounds.  With more than one score tile per block, the tensor core (a pair of tiles of 128 rows x 64 keys, D = 128: 1280
-// clocks) and the special-function unit (1024) are near each other, and what is lost is the way between them: 4096
-// new tokens at context 16384, 28 heads of 128 on 4, take 725 us = 1.16 PFLOP/s on a cool chip (60 % tensor pipe,
-// 50 % special functions active), 830 us = 1.01 PFLOP/s in a row under the power limit, where a large matrix
-// product runs at 1.4.  Keys 64 at a time with two score buffers each, because 128 at a time leave TMEM room for one (770 us).
-// Head dimension 64 has half the products for the same exponentials: 129 us for 4096 tokens, 32 heads on 8.
+// Bounds.  With more than one score tile per block, a step (64 keys for both score tiles) takes about 2050 clocks at D = 128
+// (4096 new tokens at context 16384, 28 heads of 128 on 4: 690 steps per SM in 725 us on a cool chip) and about 2200 at
+// D = 64 (4096 tokens, 32 heads on 8: 112 steps in 129 us, with the starts of the units).  The tensor core needs 1280 and
+// 640 of them, the special-function unit 1024, so neither is the limit, and half the products leave the step as long: it is
+// the way of one softmax warp from a tile's scores to the next one's, with two such warps per scheduler to fill each
+// other's gaps (issue slots 41 %, special functions 51 %, tensor pipe 60 % busy).  Clock stamps, which lengthen the step to
+// 2550, give for either D: masks, maximum and the first half of the exponentials 800, the second half 750, the way of the
+// probabilities to TMEM and their barrier 390, the barrier of the next scores 300, their way from TMEM 280.  725 us = 1.16
+// PFLOP/s; 850 us = 0.99 PFLOP/s in a row under the power limit, where a large matrix product runs at 1.4.  Keys 64 at a
+// time with two score buffers each, because 128 at a time leave TMEM room for one (770 us).
 // Single tokens are bound by HBM: 37 contexts of 8192 take 101 us = 6.2 TB/s; a few short ones by a chain of latencies
-// (19 us for four of 1300, of which the merge is 3).
+// (19 us for four of 1300, of which the merge is 3; paged_attention, one launch, has the shorter chain: 14.4).
 //
 // V tiles: a hidden key has probability 0, but 0 * inf is NaN.  Slots past the context and pages that
 // name nothing are filled with zeros (by TMA outside the tensor, by the guard warp inside a box), and
@@ -65,7 +69,8 @@ __device__ int g_ca_status = 0;
 constexpr int kOverheadTokens = 256;
 // Length per key of a block of two score tiles and of one.  Alone on the chip the one takes 1.0 us per kv tile, the
 // other 0.75 us (bound by HBM, so less beside the first): a mixed batch of 64 sequences took 265 us at 2 : 1,
-// 271 us at 3 : 2, 277 us at 5 : 4.
+// 271 us at 3 : 2, 277 us at 5 : 4.  Measured there only (28 heads of 128 on 4, caches [pages, P, Hkv, D]); head dimension
+// 64 and the other layout use the same lengths, which cost balance at most, never the result.
 constexpr int kTwoTiles = 2, kOneTile = 1;
 
 struct Line {

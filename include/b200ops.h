@@ -457,7 +457,8 @@ int b200ops_rotary(const void* q, const void* k, const int32_t* position_ids, co
  * where the position's probability is above 2^-31 of the row's largest, either of the two where it is smaller.
  * Scores, probabilities and sums are f32; for the product with V the probabilities are rounded to f16, which moves each by
  * at most 2^-11 of itself, or 2^-32 of the row's largest.
- * head_dim in {32, 64, 128, 256}; num_tokens <= 2^24.  Lengths are read on the device only, so a captured
+ * head_dim in {32, 64, 128, 256}; num_tokens <= 2^24, num_tokens * num_heads <= 2^29, bs <= 65535, num_heads <= 4096,
+ * page_size <= 2^20, max_pages_per_seq * page_size < 2^30.  Lengths are read on the device only, so a captured
  * graph serves any lengths of its shape.  Results do not depend on scheduling (bitwise repeatable).
  */
 size_t b200ops_chunked_paged_attention_workspace_size(int64_t num_tokens, int64_t bs, int64_t num_heads,
