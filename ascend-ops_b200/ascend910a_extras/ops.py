@@ -150,10 +150,16 @@ def chunked_paged_attention(
     return _C.ops.chunked_paged_attention(q, key_cache, value_cache, block_tables, context_lens, query_starts)
 
 
+def _cache_list(caches, op: str) -> list[torch.Tensor]:
+    if isinstance(caches, torch.Tensor):  # a sequence as well, of its pages
+        raise RuntimeError(f"{op}: caches must be a list of tensors, got a tensor")
+    return list(caches)
+
+
 def copy_pages(caches: list[torch.Tensor], src_pages: torch.Tensor, dst_pages: torch.Tensor) -> None:
     """caches[i][dst_pages[j]] = caches[i][src_pages[j]] for j = 0, 1, ... in order, in place; pairs
     that name no page are skipped.  `caches`: contiguous [pages, ...] tensors of any type."""
-    return _C.ops.copy_pages(list(caches), src_pages, dst_pages)
+    return _C.ops.copy_pages(_cache_list(caches, "copy_pages"), src_pages, dst_pages)
 
 
 def compact_pages(
@@ -163,4 +169,4 @@ def compact_pages(
     front of every cache, in place.  Returns (new block tables, page_map [pages]: the new number of
     each live page, -1 for the others, num_live [1]).  Every column is looked at: hand over the columns
     in use of a wide table."""
-    return _C.ops.compact_pages(list(caches), block_tables, page_counts)
+    return _C.ops.compact_pages(_cache_list(caches, "compact_pages"), block_tables, page_counts)

@@ -1,7 +1,8 @@
-"""Cache sizes that no memory has are refused, before any CUDA call."""
+"""Refusals of the page operators, before any CUDA call: sizes that no memory has, and a tensor in place of the list."""
 import ctypes
 
 import pytest
+import torch
 
 ONE = ctypes.c_void_p(256)  # never dereferenced
 NULL = ctypes.c_void_p(None)
@@ -18,3 +19,15 @@ def test_sizes_past_the_address_space(cabi, pages, size):
     need = lib.b200ops_compact_pages_workspace_size(pages)
     assert lib.b200ops_compact_pages(table, 2, pages, size, ONE, ONE, 2, 3, ctypes.c_void_p(8192), ONE, ONE,
                                      ONE, need, NULL) == cabi.EINVAL
+
+
+def test_one_tensor_in_place_of_the_list(ops):
+    """A tensor is a sequence too, of its pages: taken for the list, each page's tokens would be moved as pages."""
+    cache = torch.zeros(8, 8, 2, 16)
+    ids = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="copy_pages: caches must be a list"):
+        ops.copy_pages(cache, ids, ids)
+    with pytest.raises(RuntimeError, match="compact_pages: caches must be a list"):
+        ops.compact_pages(cache, ids[None], ids[:1])
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.copy_pages((cache,), ids, ids)
